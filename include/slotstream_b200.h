@@ -38,10 +38,15 @@ extern "C" {
 #define SSB_ERR_SLOT_RANGE 4   /* a slot index outside slot_ptr */
 #define SSB_ERR_MISALIGNED 8   /* a record base that is not 16-byte aligned */
 #define SSB_ERR_TIMEOUT 16     /* a bounded device-side wait gave up (the kernel skipped its work) */
+#define SSB_ERR_NO_PAGES 32    /* the free pages do not suffice, or a table row would overflow (nothing changed) */
+#define SSB_ERR_SEQUENCE 64    /* a sequence id out of range or named twice, a bad count, a fork onto a held sequence */
+#define SSB_ERR_PAGE_RANGE 128 /* a page id outside the pool: its tokens read as zeros, writes to it are dropped */
+#define SSB_ERR_SHARED_PAGE 256 /* new tokens would go into a page that another sequence holds too */
 
 /* ---- dtype tags for activations */
 #define SSB_BF16 0
 #define SSB_F32 1
+#define SSB_F16 2
 
 /* Library version string. */
 const char* ssb_version(void);
@@ -424,6 +429,90 @@ int ssb_gemv_affine(const void* x, int32_t x_dtype, int64_t rows, const int32_t*
  * Replaces: gemv(x, DenseWeight) of slotstream_spark/kernels/gemv_affine.py:214-262. */
 int ssb_gemv_dense(const void* x, int32_t x_dtype, int64_t rows, const uint16_t* w, int32_t n, int32_t k,
                    float* out, void* stream);
+
+/* ---- paged key-value cache (additive; the reference's attention lies outside this library's path).
+ * Keys and values of all layers of page_size consecutive tokens form one page of page_bytes bytes; pages live in
+ * `pool` [pages], and table[s * max_pages + j] is the page of tokens [j * page_size, (j + 1) * page_size) of sequence
+ * s, or -1. refs[p] counts the table entries that hold page p; bit p % 32 of free_words[p / 32] is set exactly while
+ * refs[p] is 0 (bits past `pages` are 0). lengths[s] = tokens of sequence s. All state is caller-owned device memory,
+ * read and changed in stream order: no call waits for the host, so calls can be captured. err gets SSB_ERR_* bits.
+ * scratch: int32 [ssb_kv_scratch_ints(pages, seqs)], contents irrelevant between calls; calls sharing a cache must not
+ * overlap. seqs <= 65536, pages <= 2^20, page_bytes a multiple of 16, pool 16-byte aligned. */
+typedef struct ssb_kv_cache {
+  void* pool;
+  int64_t page_bytes;
+  int32_t pages, page_size, seqs, max_pages;
+  int32_t* lengths;     /* [seqs] */
+  int32_t* refs;        /* [pages] */
+  uint32_t* free_words; /* [(pages + 31) / 32] */
+  int32_t* table;       /* [seqs, max_pages] */
+  int32_t* err;         /* [1] */
+  int32_t* scratch;
+} ssb_kv_cache;
+
+/* int32 words of scratch for a cache of `pages` pages and `seqs` sequences; SSB_EINVAL for sizes out of range. */
+int ssb_kv_scratch_ints(int32_t pages, int32_t seqs);
+
+/* lengths[ids[i]] += counts[i] for i < n, with pages for the new tokens: the entries that a sequence lacks get the
+ * lowest free pages, in the order of i and then of the entries. All or nothing: with too few free pages, a row that
+ * would pass max_pages, a bad or repeated id, a negative count, or new tokens in a page that refs says is shared,
+ * nothing changes and the error bit is set. */
+int ssb_kv_extend(const ssb_kv_cache* c, const int32_t* ids, const int32_t* counts, int32_t n, void* stream);
+
+/* Keys and values of new tokens into their pages, for one layer. Row r of k / v (16-bit elements, [rows, kv_heads, dim],
+ * strides row_stride / head_stride in elements, dim contiguous) with starts[b] <= r < starts[b + 1] is token
+ * lengths[s] - (starts[b + 1] - starts[b]) + r - starts[b] of sequence s = ids ? ids[b] : b: the newest tokens, after
+ * ssb_kv_extend. k_layer / v_layer: the layer's first element in the pool; page, head and token strides in elements.
+ * A row whose page is missing or shared is dropped, with the error bit set. Strides are multiples of 8 elements. */
+int ssb_kv_write(const ssb_kv_cache* c, const uint16_t* k, const uint16_t* v, int64_t rows, int64_t k_row_stride,
+                 int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int32_t kv_heads, int32_t dim,
+                 const int32_t* starts, const int32_t* ids, int32_t n, uint16_t* k_layer, uint16_t* v_layer,
+                 int64_t page_stride, int64_t head_stride, int64_t token_stride, void* stream);
+
+/* children[i] becomes a copy of parents[i] (i < n): full pages are shared (refs + 1), a partly filled last page is
+ * copied to a fresh page (the lowest free ones, in the order of i), so that either can be extended. A child must be
+ * empty (length 0, no pages) and named once; a parent may have many children. All or nothing, as ssb_kv_extend. */
+int ssb_kv_fork(const ssb_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
+
+/* Gives pages back: a page whose last reference goes becomes free. first / last NULL: every page of ids[i], whose
+ * length becomes 0. Otherwise pages first[i] <= j < last[i] only (entries become -1, the length stays): what a sliding
+ * window has left behind. Ids may repeat. */
+int ssb_kv_free(const ssb_kv_cache* c, const int32_t* ids, const int32_t* first, const int32_t* last, int32_t n,
+                void* stream);
+
+/* Packs the live pages into [0, live): the live pages at or past `live`, in order, are copied to the free pages below
+ * it, in order, and every table entry follows. Afterwards the free pages are [live, pages). */
+int ssb_kv_compact(const ssb_kv_cache* c, void* stream);
+
+/* ---- attention over the paged cache. Token t of a sequence is visible to the query at position p when t <= p and
+ * (window == 0 or p - t < window or t < sinks); o = sum softmax(scale * q . k) v over the visible tokens (fp32 scores,
+ * softmax statistics and sums; the softmax weights are rounded to the inputs' type for the tensor cores), zero where
+ * none is visible; lse (fp32, nullable) = log sum exp(scale * q . k), -inf there. q_type SSB_BF16 or SSB_F16, the cache
+ * and out have the same. k / v: the layer's first key and value element in the pool, with page, head and token strides
+ * in elements (multiples of 8; 16-byte aligned); pages, page_size (any), table [.., max_pages], lengths as above; ids
+ * (nullable) maps batch row b to its table row, one of table_rows (others read as empty and set
+ * SSB_ERR_SEQUENCE). What no query of the call sees is not read; a visible token whose
+ * table entry lies outside [0, pages) reads as zeros and sets SSB_ERR_PAGE_RANGE. heads is a multiple of kv_heads,
+ * query head h reads key head h / (heads / kv_heads); dim 64, 128 or 256. ws: workspace of ssb_attn_workspace bytes,
+ * contents irrelevant between calls; calls sharing it must not overlap.
+ *
+ * ssb_attn_decode: q [n, q_len, heads, dim] (strides in elements, multiples of 8), the q_len newest tokens of each
+ * sequence (positions lengths - q_len ..; a position below 0 has no visible token). q_len * heads / kv_heads <= 128.
+ * ssb_attn_prefill: ragged q [rows, heads, dim]; rows starts[b] <= r < starts[b + 1] are the newest tokens of
+ * sequence b. out / lse are contiguous. */
+int ssb_attn_workspace(int32_t dim, int32_t n, int32_t prefill, int64_t rows, int32_t heads, int64_t* bytes);
+int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride,
+                    const void* k, const void* v, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                    int32_t n, int32_t q_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t page_size,
+                    int32_t pages, const int32_t* table, int32_t table_rows, int32_t max_pages, const int32_t* lengths,
+                    const int32_t* ids, int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
+                    int64_t ws_bytes, int32_t* err, void* stream);
+int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+                     const void* v, int64_t page_stride, int64_t head_stride, int64_t token_stride, int64_t rows,
+                     const int32_t* starts, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim, int32_t page_size,
+                     int32_t pages, const int32_t* table, int32_t table_rows, int32_t max_pages, const int32_t* lengths,
+                     const int32_t* ids, int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
+                     int64_t ws_bytes, int32_t* err, void* stream);
 
 #ifdef __cplusplus
 }

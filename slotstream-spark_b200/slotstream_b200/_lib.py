@@ -13,7 +13,8 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libslotstream_b200.so"
 
 SSB_OK, SSB_EINVAL, SSB_EUNSUPPORTED, SSB_ENODEVICE, SSB_ETOOBIG, SSB_ETIMEDOUT = 0, -1, -2, -3, -4, -5
 ERR_EXPERT_RANGE, ERR_UNMAPPED, ERR_SLOT_RANGE, ERR_MISALIGNED, ERR_TIMEOUT = 1, 2, 4, 8, 16
-BF16, F32 = 0, 1
+ERR_NO_PAGES, ERR_SEQUENCE, ERR_PAGE_RANGE, ERR_SHARED_PAGE = 32, 64, 128, 256
+BF16, F32, F16 = 0, 1, 2
 ROUTER_ROUND_BF16, ROUTER_SHARED_GATE = 1, 2
 DECODE_PDL = 1
 DECODE_FUSED_CUDA_CORES = 4
@@ -22,6 +23,15 @@ DECODE_FUSED_TENSOR_CORES = 8
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
+_F32 = ctypes.c_float
+
+
+class KvCacheStruct(ctypes.Structure):
+    """ssb_kv_cache of the C header."""
+    _fields_ = [("pool", _P), ("page_bytes", _I64), ("pages", _I32), ("page_size", _I32), ("seqs", _I32),
+                ("max_pages", _I32), ("lengths", _P), ("refs", _P), ("free_words", _P), ("table", _P), ("err", _P),
+                ("scratch", _P)]
+
 
 # name -> argtypes (every entry point returns int)
 SIGNATURES = {
@@ -75,6 +85,17 @@ SIGNATURES = {
     "ssb_sorted_gate_up": [_P, _I32, _I32, _P, _I64, _P, _P, _P, _I64, _P, _I32, _I32, _P, _P, _P],
     "ssb_sorted_down": [_P, _I64, _I32, _I32, _P, _P, _P, _P, _I64, _P, _I32, _I32, _P, _P, _P],
     "ssb_gemm_dense": [_P, _I64, _I32, _P, _I32, _P, _I64, _P],
+    "ssb_kv_scratch_ints": [_I32, _I32],
+    "ssb_kv_extend": [_P, _P, _P, _I32, _P],
+    "ssb_kv_write": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P],
+    "ssb_kv_fork": [_P, _P, _P, _I32, _P],
+    "ssb_kv_free": [_P, _P, _P, _P, _I32, _P],
+    "ssb_kv_compact": [_P, _P],
+    "ssb_attn_workspace": [_I32, _I32, _I32, _I64, _I32, _P],
+    "ssb_attn_decode": [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
+                        _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
+    "ssb_attn_prefill": [_P, _I32, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32,
+                         _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
 }
 
 _lib = None

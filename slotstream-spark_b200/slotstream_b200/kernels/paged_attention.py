@@ -1,0 +1,122 @@
+"""Attention over a paged key-value cache (additive API): decode steps and ragged prompts.
+
+The reference's attention lies outside the path that this package replaces; these entry points give the layers between
+the MoE layers. ``k_pages`` / ``v_pages`` are [pages, kv_heads, page_size, head_dim] (bf16 or fp16, any strides that are
+multiples of 8 with the last dimension contiguous, equal for both), e.g. ``PagedKvCache.k(layer)`` / ``v(layer)``;
+``page_table`` int32 [rows, max_pages]; ``lengths`` int32 [rows] counts the tokens in the cache, the queries' own among
+them. The queries of a sequence are its newest tokens, so query i of q sits at position lengths - q + i; it sees the
+tokens t at or before it, and where ``window`` > 0 only those less than ``window`` back, and the first ``sinks``.
+A query that sees nothing gives zeros and a log-sum-exp of -inf. ``ids`` (int32) maps batch row b to its table row.
+
+Scores, softmax statistics and sums are fp32; the softmax weights are rounded to the inputs' type for the tensor cores.
+``lse`` (fp32, optional output) is the natural log-sum-exp of the scaled scores, for joining with other parts. ``err``
+(int32 [1], e.g. ``PagedKvCache.err``) gets error bits; ``ws`` (uint8, ``workspace_bytes``) avoids the allocation of a
+workspace, which capture in a CUDA graph with caller-owned memory wants."""
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_WS = {}
+
+
+def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, prefill: bool = False) -> int:
+    """Bytes of ``ws`` for ``n`` sequences with ``rows`` query tokens in all."""
+    key = (head_dim, n, rows, heads, prefill, torch.cuda.current_device())
+    got = _WS.get(key)
+    if got is None:
+        b = ctypes.c_int64()
+        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, int(prefill), rows, heads, ctypes.byref(b)),
+                   "attention workspace")
+        if len(_WS) > 4096:
+            _WS.clear()
+        got = _WS[key] = b.value
+    return got
+
+
+def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse):
+    tag = _TYPES.get(q.dtype)
+    if tag is None or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise ValueError("q, k_pages and v_pages must all be bf16 or all fp16")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != dim:
+        raise ValueError(f"k_pages and v_pages must both be [pages, kv_heads, page_size, {dim}]")
+    ks = k_pages.stride()
+    if ks != v_pages.stride() or ks[3] != 1:
+        raise ValueError("k_pages and v_pages must have the same strides, the last one 1")
+    if heads % k_pages.shape[1]:
+        raise ValueError(f"{heads} query heads are no multiple of {k_pages.shape[1]} key heads")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 [rows, max_pages]")
+    rows = page_table.shape[0]
+    if lengths.dtype != torch.int32 or lengths.shape != (rows,) or not lengths.is_contiguous():
+        raise ValueError("lengths must be a contiguous int32 vector, one per row of page_table")
+    if ids is not None:
+        if ids.dtype != torch.int32 or ids.shape != (n,) or not ids.is_contiguous():
+            raise ValueError(f"ids must be a contiguous int32 vector of {n}")
+    elif n > rows:
+        raise ValueError(f"{n} sequences, but page_table has {rows} rows")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    if err is not None and (err.dtype != torch.int32 or err.numel() != 1):
+        raise ValueError("err must be one int32")
+    shape = q.shape
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
+        raise ValueError("out must be contiguous, with q's shape and type")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:-1] or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous fp32 tensor of q's shape without the last dimension")
+    return tag, ks, rows, out
+
+
+def _workspace(ws, dim, n, rows, heads, prefill, device):
+    need = workspace_bytes(dim, n, rows, heads, prefill)
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=device), need
+    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
+        raise ValueError(f"ws must be a contiguous uint8 tensor of at least {need} bytes")
+    return ws, ws.numel()
+
+
+def attn_decode(q, k_pages, v_pages, page_table, lengths, out=None, *, lse=None, scale=None, window: int = 0,
+                sinks: int = 0, ids=None, err=None, ws=None):
+    """q [n, q_len, heads, head_dim] -> out of the same shape: the ``q_len`` newest tokens of every sequence (one of a
+    decode step, a few of a speculative verify; q_len * heads / kv_heads <= 128). ``scale`` defaults to
+    1 / sqrt(head_dim)."""
+    if q.dim() != 4 or q.stride(3) != 1:
+        raise ValueError("q must be [n, q_len, heads, head_dim] with a contiguous head_dim")
+    n, q_len, heads, dim = q.shape
+    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse)
+    ws, ws_bytes = _workspace(ws, dim, n, n * q_len, heads, False, q.device)
+    p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
+    rc = _lib.lib().ssb_attn_decode(
+        p(q), tag, qs[0], qs[1], qs[2], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], n, q_len, heads, kp[1], dim, kp[2],
+        kp[0], p(page_table), rows, page_table.shape[1], p(lengths), p(ids), window, sinks,
+        1.0 / math.sqrt(dim) if scale is None else scale, p(out), p(lse), p(ws), ws_bytes, p(err), _lib.stream())
+    _lib.check(rc, "attn_decode")
+    return out
+
+
+def attn_prefill(q, k_pages, v_pages, page_table, lengths, starts, out=None, *, lse=None, scale=None, window: int = 0,
+                 sinks: int = 0, ids=None, err=None, ws=None):
+    """q [rows, heads, head_dim] -> out of the same shape. Rows ``starts[b]`` to ``starts[b + 1]`` (int32 [n + 1], on the
+    device, rising) are the newest tokens of sequence b: whole prompts, or chunks after cached ones. Rows outside
+    every sequence are not written."""
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be [rows, heads, head_dim] with a contiguous head_dim")
+    if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
+        raise ValueError("starts must be a contiguous int32 vector of at least one element")
+    total, heads, dim = q.shape
+    n = starts.numel() - 1
+    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse)
+    ws, ws_bytes = _workspace(ws, dim, n, total, heads, True, q.device)
+    p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
+    rc = _lib.lib().ssb_attn_prefill(
+        p(q), tag, qs[0], qs[1], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], total, p(starts), n, heads, kp[1], dim,
+        kp[2], kp[0], p(page_table), rows, page_table.shape[1], p(lengths), p(ids), window, sinks,
+        1.0 / math.sqrt(dim) if scale is None else scale, p(out), p(lse), p(ws), ws_bytes, p(err), _lib.stream())
+    _lib.check(rc, "attn_prefill")
+    return out

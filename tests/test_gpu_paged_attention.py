@@ -1,0 +1,206 @@
+"""Attention over the paged cache against its definition in 64 bits (GPU)."""
+import numpy as np
+import pytest
+import torch
+
+from paged_reference import assert_attention, attention
+from slotstream_b200.kernels.paged_attention import attn_decode, attn_prefill, workspace_bytes
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _cache(lengths, kv, dim, ps, dtype, seed=0, layers=2, layer=1, spare=3):
+    """Pages dealt at random, the slots past each length filled with NaN; returns strided k / v views and the table."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    held = [-(-n // ps) for n in lengths]
+    pages, mp = sum(held) + spare, max(held + [1]) + 1
+    pool = torch.full((pages, layers, 2, kv, ps, dim), float("nan"), dtype=dtype, device="cuda")
+    order = np.random.default_rng(seed).permutation(pages)
+    table = np.full((len(lengths), mp), -1, np.int32)
+    at = 0
+    for s, (n, h) in enumerate(zip(lengths, held)):
+        table[s, :h] = order[at:at + h]
+        at += h
+        for j in range(h):
+            m = min(ps, n - j * ps)
+            pool[int(table[s, j]), layer, :, :, :m] = torch.randn(2, kv, m, dim, device="cuda", generator=g,
+                                                                  dtype=torch.float32).to(dtype)
+    return (pool[:, layer, 0], pool[:, layer, 1], torch.from_numpy(table).cuda(),
+            torch.tensor(lengths, dtype=torch.int32, device="cuda"), g)
+
+
+def _q(g, rows, heads, kv, dim, dtype):
+    """Queries inside a wider projection output: strided, not contiguous."""
+    both = torch.randn(rows, heads + 2 * kv, dim, device="cuda", generator=g, dtype=torch.float32).to(dtype)
+    return both[:, :heads] * 1 if rows == 0 else both[:, :heads]
+
+
+def _decode(lengths, q_len, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0):
+    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed)
+    n = len(lengths)
+    q = _q(g, n * q_len, heads, kv, dim, dtype)
+    lse = torch.full((n, q_len, heads), 7.0, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attn_decode(q.unflatten(0, (n, q_len)), k, v, table, lens, lse=lse, window=window, sinks=sinks, err=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    assert_attention(out.flatten(0, 1), lse.flatten(0, 1), attention(q, k, v, table, lens, [q_len] * n, window, sinks))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv", [(8, 1), (6, 2), (4, 4), (40, 2)])
+def test_decode_one_token(dtype, dim, heads, kv):
+    _decode([1, 0, 17, 300, 1025], 1, heads, kv, dim, 16, dtype)
+
+
+@pytest.mark.parametrize("ps", [1, 5, 8, 24, 100, 128])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_decode_page_sizes(ps, dim):
+    _decode([333, 64, ps, ps + 1, 2 * ps - 1], 1, 8, 2, dim, ps, BF)
+
+
+@pytest.mark.parametrize("q_len", [1, 2, 3, 5])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (100, 4), (64, 70), (5000, 4)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_window_and_verify(q_len, window, sinks, dim):
+    _decode([0, 1, 2, 130, 700, 1111], q_len, 12, 2, dim, 24, BF, window, sinks)
+
+
+def test_decode_rows_past_a_tile():
+    """64 and 128 query rows per key head: several row blocks."""
+    _decode([500, 3], 4, 32, 2, 128, 16, HF)
+    _decode([500, 3], 8, 16, 1, 256, 16, BF, 100, 4)
+
+
+def test_decode_many_sequences_and_a_long_one():
+    rng = np.random.default_rng(3)
+    _decode([9000] + rng.integers(0, 40, 300).tolist(), 1, 4, 2, 128, 16, BF)
+    _decode([20011], 1, 2, 1, 64, 32, HF)
+
+
+def _prefill(lengths, new, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0, ids=None):
+    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed)
+    rows = sum(new)
+    q = _q(g, rows, heads, kv, dim, dtype)
+    starts = torch.from_numpy(np.cumsum([0] + new).astype(np.int32)).cuda()
+    lse = torch.full((rows, heads), 7.0, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    idt = None if ids is None else torch.tensor(ids, dtype=torch.int32, device="cuda")
+    out = attn_prefill(q, k, v, table, lens, starts, lse=lse, window=window, sinks=sinks, err=err, ids=idt)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    assert_attention(out, lse, attention(q, k, v, table, lens, new, window, sinks, ids=ids))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2), (8, 1), (5, 1)])
+def test_prefill_ragged(dtype, dim, heads, kv):
+    _prefill([1, 37, 130, 257, 5], [1, 37, 129, 100, 0], heads, kv, dim, 16, dtype)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 4), (100, 0), (128, 300), (4000, 1)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prefill_window(window, sinks, dim):
+    _prefill([700, 300], [513, 300], 4, 2, dim, 24, BF, window, sinks)
+
+
+@pytest.mark.parametrize("ps", [1, 7, 64, 200])
+def test_prefill_page_sizes_and_ids(ps):
+    _prefill([300, 50, 411], [40, 411], 4, 1, 128, ps, BF, ids=[1, 2])
+
+
+def test_prefill_long_context_few_rows():
+    _prefill([9001], [3], 4, 2, 128, 32, BF)
+    _prefill([6000], [17], 16, 2, 256, 16, HF, 5000, 8)
+
+
+def test_prefill_more_queries_than_tokens_sees_nothing():
+    _prefill([3, 0], [8, 4], 4, 2, 64, 16, BF)
+
+
+def test_ids_choose_table_rows_and_bad_ids_read_as_empty():
+    k, v, table, lens, g = _cache([40, 90, 17], 2, 64, 16, BF)
+    q = _q(g, 3, 4, 2, 64, BF).unflatten(0, (3, 1))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ids = torch.tensor([2, 5, 0], dtype=torch.int32, device="cuda")
+    out = attn_decode(q, k, v, table, lens, ids=ids, err=err)
+    ref = attn_decode(q[[0, 2]].contiguous(), k, v, table[[2, 0]].contiguous(), lens[[2, 0]].contiguous())
+    assert torch.equal(out[[0, 2]], ref) and bool((out[1] == 0).all())
+    assert int(err.item()) == 64
+
+
+def test_missing_page_reads_as_zeros_and_is_reported():
+    k, v, table, lens, g = _cache([70], 1, 64, 16, BF)
+    q = _q(g, 1, 4, 1, 64, BF).unflatten(0, (1, 1))
+    bad = table.clone()
+    bad[0, 1] = 10 ** 6
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attn_decode(q, k, v, bad, lens, err=err)
+    assert int(err.item()) == 128
+    pool = torch.zeros_like(k[:1])
+    k2, v2 = torch.cat([k, pool]), torch.cat([v, pool])
+    bad[0, 1] = k2.shape[0] - 1
+    ref = attention(q[0], k2, v2, bad, lens, [1])
+    assert bool(((out[0].double() - ref[0]).abs() <= ref[2]).all())
+
+
+def test_pages_behind_the_window_are_not_read():
+    """The pages between the sinks and the window may be gone (-1): no error, the same result."""
+    k, v, table, lens, g = _cache([700], 2, 128, 16, BF)
+    q = _q(g, 1, 4, 2, 128, BF).unflatten(0, (1, 1))
+    full = attn_decode(q, k, v, table, lens, window=100, sinks=4)
+    gone = table.clone()
+    gone[0, 1:(700 - 100) // 16] = -1
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(attn_decode(q, k, v, gone, lens, window=100, sinks=4, err=err), full)
+    assert int(err.item()) == 0
+
+
+def test_results_repeat_and_a_batch_equals_itself_in_a_graph():
+    k, v, table, lens, g = _cache([700, 30, 2000], 2, 128, 16, BF)
+    q = _q(g, 3, 16, 2, 128, BF).unflatten(0, (3, 1))
+    ws = torch.empty(workspace_bytes(128, 3, 3, 16), dtype=torch.uint8, device="cuda")
+    out, ref = torch.empty(q.shape, dtype=BF, device="cuda"), attn_decode(q, k, v, table, lens)
+    graph = torch.cuda.CUDAGraph()
+    attn_decode(q, k, v, table, lens, out, ws=ws)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        attn_decode(q, k, v, table, lens, out, ws=ws)
+    for _ in range(3):
+        out.zero_()
+        ws.fill_(255)                       # what an earlier call left in the workspace does not matter
+        graph.replay()
+        assert torch.equal(out, ref)
+
+
+def test_on_a_side_stream():
+    k, v, table, lens, g = _cache([700, 30], 2, 64, 16, HF)
+    q = _q(g, 2, 4, 2, 64, HF).unflatten(0, (2, 1))
+    ref = attn_decode(q, k, v, table, lens)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        out = attn_decode(q, k, v, table, lens)
+    side.synchronize()
+    assert torch.equal(out, ref)
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 elements, the sequence at its end."""
+    ps, kv, dim = 16, 8, 128
+    pages = 2 ** 32 // (2 * ps * kv * dim) + 5
+    pool = torch.empty(pages, 1, 2, kv, ps, dim, dtype=BF, device="cuda")
+    pool[-3:] = torch.randn(3, 1, 2, kv, ps, dim, device="cuda").to(BF)
+    table = torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([43], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 1, 16, dim, device="cuda").to(BF)
+    lse = torch.empty(1, 1, 16, device="cuda")
+    for out in (attn_decode(q, pool[:, 0, 0], pool[:, 0, 1], table, lens, lse=lse),
+                attn_prefill(q[0], pool[:, 0, 0], pool[:, 0, 1], table, lens,
+                             torch.tensor([0, 1], dtype=torch.int32, device="cuda"), lse=lse[0])[None]):
+        assert_attention(out[0], lse[0], attention(q[0], pool[:, 0, 0], pool[:, 0, 1], table, lens, [1]))
+    del pool
+    torch.cuda.empty_cache()
