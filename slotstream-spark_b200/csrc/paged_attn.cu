@@ -443,7 +443,7 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
          int32_t* err) {
   SSB_CHECK_ARG(q_type == SSB_BF16 || q_type == SSB_F16);
   SSB_CHECK_ARG(n >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && page_size > 0 && pages > 0 &&
-                table_rows > 0 && max_pages > 0 && window >= 0 && sinks >= 0);
+                table_rows > 0 && max_pages > 0 && window >= 0 && sinks >= 0 && scale > 0.f && scale <= 3.4e38f);
   SSB_CHECK_ARG((int64_t)max_pages * page_size <= 0x7FFFFFFFll - 1024 && sinks <= 0x7FFFFFFF - 1024);
   if (dim != 64 && dim != 128 && dim != 256) return SSB_EUNSUPPORTED;
   SSB_CHECK_ARG((page_stride | head_stride | token_stride) % 8 == 0);
@@ -484,12 +484,16 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
 
 using namespace attn;
 
-extern "C" int ssb_attn_workspace(int32_t dim, int32_t n, int32_t prefill, int64_t rows, int32_t heads,
-                                  int64_t* bytes) {
-  SSB_CHECK_ARG(bytes && n >= 0 && rows >= 0 && heads > 0);
-  (void)prefill;
+static int64_t workspace(int dim, int n, int64_t rows, int heads, int kv_heads, bool prefill) {
+  return prefill ? prefill_workspace(dim, n, rows, heads, kv_heads) : layout_of(blocks_of(dim), RB, dim).bytes;
+}
+
+extern "C" int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads,
+                                  int32_t prefill, int64_t* bytes) {
+  SSB_CHECK_ARG(bytes && n >= 0 && rows >= 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0);
+  SSB_CHECK_ARG(rows * (heads / kv_heads) < (1ll << 30));
   if (dim != 64 && dim != 128 && dim != 256) return SSB_EUNSUPPORTED;
-  *bytes = layout_of(blocks_of(dim), RB, dim).bytes;
+  *bytes = workspace(dim, n, rows, heads, kv_heads, prefill != 0);
   return SSB_OK;
 }
 
@@ -532,11 +536,10 @@ extern "C" int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_str
   SSB_CHECK_ARG(rows >= 0 && rows * (heads / kv_heads) < (1ll << 30) && (q_tok_stride | q_head_stride) % 8 == 0);
   if (n == 0 || rows == 0) return SSB_OK;
   SSB_CHECK_ARG(q && k && v && table && lengths && starts && out && ws);
-  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= layout_of(blocks_of(dim), RB, dim).bytes);
+  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= workspace(dim, n, rows, heads, kv_heads, true));
   a.q_tok = q_tok_stride;
   a.q_head = q_head_stride;
   a.starts = starts;
   a.rows = rows;
-  return q_type == SSB_BF16 ? launch_dim<__nv_bfloat16>(a, dim, (uint8_t*)ws, (cudaStream_t)stream)
-                            : launch_dim<__half>(a, dim, (uint8_t*)ws, (cudaStream_t)stream);
+  return prefill_launch(a, dim, q_type == SSB_BF16, ws, stream);
 }

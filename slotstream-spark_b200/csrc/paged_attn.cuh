@@ -105,4 +105,8 @@ SSB_DEV float ex2(float x) {
 }
 constexpr float LN2 = 0.6931471805599453f;
 
+// csrc/paged_prefill.cu
+int64_t prefill_workspace(int dim, int n, int64_t rows, int heads, int kv_heads);
+int prefill_launch(Args& a, int dim, bool bf16, void* ws, void* stream);
+
 }  // namespace attn

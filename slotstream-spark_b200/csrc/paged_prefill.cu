@@ -1,0 +1,714 @@
+// Attention over the paged key-value cache for prompts: causal, ragged, with a sliding window and sinks.
+//
+// The rows of one key head are (query token, head of its group) pairs, flattened; an item is MB = 128 NT of them
+// against the tokens they can see, in tiles of T tokens. Per tile, on the tensor cores (tcgen05, fp32 in TMEM):
+// S = Q K^T from shared memory, and O += P V with P read from TMEM, where the softmax has put it.
+// What bounds it: the two products are 4 T MB D operations and the softmax T MB exponentials per tile; at head size
+// 128 the tensor cores and the 16 exponentials per clock of an SM need the same time, so both have to run all the time.
+// Hence two row tiles of 128 in turn (NT = 2): while one is in the softmax the other is in the products. At head size 256
+// one accumulator fills half of TMEM, so one row tile (NT = 1) alternates between two buffers of S instead: S of
+// the next tile is computed while the softmax works on this one.
+//
+// The running maximum is only raised when a row's maximum grows by more than 2^8 (log2 domain): p stays below 2^8, which
+// both types and the fp32 sums hold with the same relative precision, and rescaling the accumulator in TMEM becomes rare.
+//
+// Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V rows through
+// cp.async (any page size; rows that no query sees become zeros) into 128-byte-swizzled tiles, and one that issues
+// the matrix instructions; one lane of another hands out units. The two products have different shapes or accumulators, so
+// nothing orders them but the waits here: P has columns of its own where TMEM has room (head sizes 64 and 256); at 128
+// it takes the place of S, and the next S is not started before the product that reads P has finished.
+//
+// Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
+// (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
+// take units from the list by a counter. Only the items of the last wave or so are cut, and k_prefill_join sums their
+// pieces in order, so the outcome does not depend on who took which.
+#include "paged_attn.cuh"
+
+#include "affine.cuh"
+#include "tc_common.cuh"
+
+namespace attn {
+namespace {
+
+template <int D>
+struct Cfg {
+  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 256 ? 64 : 128, SLOTS = D == 64 ? 8 : 5;
+  static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
+  static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
+  // TMEM columns: the accumulators, two buffers of S, two of P (two elements a column)
+  static constexpr bool P_IN_S = D == 128;
+  static constexpr int S_COL = NT * D, P_COL = P_IN_S ? S_COL : S_COL + 2 * T, P_STEP = P_IN_S ? T : T / 2;
+  static_assert((P_IN_S ? S_COL : P_COL) + (P_IN_S ? 2 * T : T) <= 512, "TMEM");
+};
+constexpr int PLAN_T = 1024, LAG = 3;
+
+struct __align__(16) Unit {
+  int b, h, r0, rows;          // sequence, key head, first flat row, rows
+  int i0, i1, len, q;          // tiles of the unit, sequence length, query tokens
+  int q0, row, slot, pad;      // first query token, table row, piece slot (-1: a whole item)
+};
+struct __align__(16) Joint {
+  int h, r0, rows, q0, slot, pieces, pad0, pad1;
+};
+
+struct Work {
+  int* item0;                  // [n + 1] first item of each sequence
+  int* ctl;                    // [0] units taken, [1] units, [2] joints
+  Unit* units;
+  Joint* joints;
+  int max_units, max_slots;
+};
+
+SSB_DEV int block_scan(int v, int* part, int* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    int u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();
+  if (lane == 31) part[w] = inc;
+  __syncthreads();
+  if (w == 0) {
+    const int p = part[lane];
+    int q = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      int u = __shfl_up_sync(0xFFFFFFFFu, q, o);
+      if (lane >= o) q += u;
+    }
+    part[lane] = q - p;
+    if (lane == 31) part[32] = q;
+  }
+  __syncthreads();
+  *total = part[32];
+  return part[w] + inc - v;
+}
+SSB_DEV long long block_scan_ll(long long v, long long* part, long long* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    long long u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();
+  if (lane == 31) part[w] = inc;
+  __syncthreads();
+  if (w == 0) {
+    const long long p = part[lane];
+    long long q = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      long long u = __shfl_up_sync(0xFFFFFFFFu, q, o);
+      if (lane >= o) q += u;
+    }
+    part[lane] = q - p;
+    if (lane == 31) part[32] = q;
+  }
+  __syncthreads();
+  *total = part[32];
+  return part[w] + inc - v;
+}
+
+struct ItemAt {
+  int b, h, r0, rows, tiles, len, q, q0, row;
+};
+// Item i: sequences in order, key heads inside, row blocks from the last one (the longest) down.
+template <int MB, int T>
+SSB_DEV ItemAt item_at(const Args& a, const Work& w, int i) {
+  int lo = 0, hi = a.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (w.item0[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  const Seq s = seq_of(a, lo);
+  const int flat = s.q * a.group, nb = (flat + MB - 1) / MB, k = i - w.item0[lo];
+  ItemAt t;
+  t.b = lo;
+  t.h = k / nb;
+  t.r0 = (nb - 1 - (k - t.h * nb)) * MB;
+  t.rows = min(MB, flat - t.r0);
+  const int p = s.len - s.q;
+  t.tiles = range_of(a, p + t.r0 / a.group, p + (t.r0 + t.rows - 1) / a.group, T).tiles;
+  t.len = s.len;
+  t.q = s.q;
+  t.q0 = (int)s.q0;
+  t.row = s.row;
+  return t;
+}
+
+template <int MB, int T>
+__global__ void __launch_bounds__(PLAN_T) k_prefill_plan(Args a, Work w, int blocks) {
+  __shared__ int part[33];
+  __shared__ long long lpart[33];
+  int items = 0;
+  for (int b0 = 0; b0 < a.n; b0 += PLAN_T) {
+    const int b = b0 + threadIdx.x;
+    int c = 0;
+    if (b < a.n) {
+      const Seq s = seq_of(a, b);
+      if (s.row < 0 && s.q > 0) set_err(a.err, SSB_ERR_SEQUENCE);
+      c = a.kv_heads * ((s.q * a.group + MB - 1) / MB);
+    }
+    int total;
+    const int ex = block_scan(c, part, &total);
+    if (b < a.n) w.item0[b] = items + ex;
+    items += total;
+  }
+  if (threadIdx.x == 0) w.item0[a.n] = items;
+  __syncthreads();
+  items = min(items, w.max_units);                      // starts that overlap would list more: never out of bounds
+  long long all = 0;
+  for (int i = threadIdx.x; i < items; i += PLAN_T) all += item_at<MB, T>(a, w, i).tiles;
+  long long sum;
+  block_scan_ll(all, lpart, &sum);
+  const long long least = max(sum / (16ll * blocks), 2ll);
+  long long before = 0;
+  int units = 0, slots = 0, joints = 0;
+  for (int i0 = 0; i0 < items; i0 += PLAN_T) {
+    const int i = i0 + threadIdx.x;
+    ItemAt t = {};
+    if (i < items) t = item_at<MB, T>(a, w, i);
+    long long total;
+    const long long ex = block_scan_ll(t.tiles, lpart, &total);
+    const long long left = sum - before - ex;
+    before += total;
+    const long long most = max(left / blocks, least);
+    int k = i < items ? (int)((t.tiles + most - 1) / most) : 0;
+    int n_s, n_j, n_u;
+    const int at = slots + block_scan(k > 1 ? k : 0, part, &n_s);
+    const bool cut = k > 1 && at + k <= w.max_slots;
+    if (k > 1 && !cut) k = 1;
+    const int j = joints + block_scan(cut, part, &n_j), u = units + block_scan(k, part, &n_u);
+    if (cut) w.joints[j] = Joint{t.h, t.r0, t.rows, t.q0, at, k, 0, 0};
+    for (int x = 0; x < k; ++x)
+      w.units[u + x] = Unit{t.b, t.h, t.r0, t.rows, (int)((long long)t.tiles * x / k), (int)((long long)t.tiles * (x + 1) / k),
+                            t.len, t.q, t.q0, t.row, cut ? at + x : -1, 0};
+    slots += n_s;
+    joints += n_j;
+    units += n_u;
+  }
+  if (threadIdx.x == 0) {
+    w.ctl[0] = 0;
+    w.ctl[1] = units;
+    w.ctl[2] = joints;
+  }
+}
+
+// mbar_wait_ns by a whole warp that goes on to warp-wide TMEM instructions: the lanes may leave the wait one by one, and
+// the vote brings them together again.
+SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_ns(bar, parity & 1, SSB_WAIT_NS));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column.
+SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of a tile whose rows are the K index (tokens) and whose 128-byte swizzled panels hold 64 of the N index:
+// panels `panel` bytes apart, groups of eight tokens 1024 bytes apart.
+SSB_DEV uint64_t umma_desc_mn(uint32_t smem_addr, uint32_t panel) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(panel >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+template <typename E>
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn);
+template <>
+constexpr uint32_t idesc_of<__nv_bfloat16>(int m, int n, bool b_mn) {
+  return idesc_bf16_f32(m, n) | (b_mn ? 1u << 16 : 0u);
+}
+template <>
+constexpr uint32_t idesc_of<__half>(int m, int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+SSB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+SSB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename E, int D>
+__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) {
+  using C = Cfg<D>;
+  constexpr int NT = C::NT, T = C::T, CPR = C::CPR, SLOTS = C::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sq = smem;
+  uint8_t* ring = smem + C::QB;
+  uint64_t* bar = (uint64_t*)(ring + SLOTS * C::SLOT);
+  uint64_t *q_full = bar, *q_empty = bar + 1, *s_full = bar + 2, *p_full = bar + 4, *o_done = bar + 6, *u_full = bar + 8,
+           *u_empty = bar + 10, *full = bar + 12, *empty = full + SLOTS;
+  int* u_slot = (int*)(empty + SLOTS);             // unit numbers handed out, two in flight
+  uint32_t* tmem_slot = (uint32_t*)(u_slot + 2);
+  int* failed = (int*)(tmem_slot + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (smem_u32(smem) & 1023u) {                     // the swizzled tiles need it; the same for every thread
+    if (tid == 0) set_err(a.err, SSB_ERR_MISALIGNED);
+    return;
+  }
+  constexpr int PROD = NT * 4, MMA = PROD + 4, SCHED = MMA + 1;      // first warps of the roles
+
+  if (warp == MMA) tmem_alloc(tmem_slot, 512);
+  if (tid == 0) {
+    mbar_init(q_full, 128);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_done + i, 1);
+      mbar_init(u_full + i, 1);
+      mbar_init(u_empty + i, NT * 128 + 128 + 1);
+    }
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(full + i, 128);
+      mbar_init(empty + i, 1);
+    }
+    *failed = 0;
+    fence_mbar_init();
+  }
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto give_up = [&] { atomicExch(failed, 1); };
+  int un = 0;                                       // units this thread has seen
+  // The next unit, or false at the end of the list (or when a wait gave up).
+  auto next_unit = [&](Unit& u) {
+    const int s = un & 1;
+    if (!mbar_wait_ns(u_full + s, (un >> 1) & 1, SSB_WAIT_NS)) {
+      give_up();
+      return false;
+    }
+    const int i = *(volatile int*)(u_slot + s);
+    mbar_arrive(u_empty + s);
+    ++un;
+    if (i < 0) return false;
+    u = w.units[i];
+    return true;
+  };
+  auto range_for = [&](const Unit& u) {
+    const int p = u.len - u.q;
+    return range_of(a, p + u.r0 / a.group, p + (u.r0 + u.rows - 1) / a.group, T);
+  };
+
+  if (warp == SCHED) {
+    if (lane == 0) {
+      const int units = w.ctl[1];
+      for (int k = 0;; ++k) {
+        const int s = k & 1;
+        if (k >= 2 && !mbar_wait_ns(u_empty + s, ((k >> 1) - 1) & 1, SSB_WAIT_NS)) {
+          give_up();
+          break;
+        }
+        const int i = *(volatile int*)failed ? units : atomicAdd(w.ctl, 1);
+        *(volatile int*)(u_slot + s) = i < units ? i : -1;
+        mbar_arrive(u_full + s);
+        if (i >= units) break;
+      }
+    }
+  } else if (warp == MMA) {
+    if (lane == 0) {
+      constexpr uint32_t ID_S = idesc_of<E>(128, T, false), ID_O = idesc_of<E>(128, D, true);
+      Unit u;
+      uint32_t kv = 0, qn = 0, tn = 0;              // slots, units and tiles so far
+      bool ok = true;
+      auto scores = [&](int t, int buf, uint32_t slot) {
+        const uint32_t ks = smem_u32(ring + (slot % SLOTS) * C::SLOT), qs = smem_u32(sq);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(tmem + C::S_COL + buf * T, umma_desc_sw128(qs + (k / 4) * (C::MB * 128) + t * 128 * 128 + (k % 4) * 32),
+                    umma_desc_sw128(ks + (k / 4) * (T * 128) + (k % 4) * 32), ID_S, k > 0);
+        umma_commit(s_full + buf);
+      };
+      auto outputs = [&](int t, int buf, uint32_t slot, bool first) {
+        const uint32_t vs = smem_u32(ring + (slot % SLOTS) * C::SLOT);
+#pragma unroll
+        for (int k = 0; k < T / 16; ++k)
+          umma_ts(tmem + t * D, tmem + C::P_COL + buf * C::P_STEP + k * 8, umma_desc_mn(vs + k * 2048, T * 128), ID_O, !first || k > 0);
+        umma_commit(o_done + t);
+      };
+      auto need = [&](uint64_t* b, uint32_t parity) {
+        if (ok && !mbar_wait_ns(b, parity & 1, SSB_WAIT_NS)) ok = false;
+        if (ok) tc_fence_after();
+        return ok;
+      };
+      while (ok && next_unit(u)) {
+        const int n = u.i1 - u.i0;
+        if (!need(q_full, qn) || !need(full + kv % SLOTS, kv / SLOTS)) break;
+        if constexpr (NT == 2) {
+          if (C::P_IN_S && tn && (!need(o_done, tn - 1) || !need(o_done + 1, tn - 1))) break;
+          scores(0, 0, kv);
+          scores(1, 1, kv);
+          umma_commit(empty + kv % SLOTS);
+          if (n == 1) umma_commit(q_empty);
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t vslot = kv + 2 * j + 1, kslot = vslot + 1;
+            if (!need(full + vslot % SLOTS, vslot / SLOTS)) break;
+            if (j + 1 < n && !need(full + kslot % SLOTS, kslot / SLOTS)) break;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!need(p_full + t, tn + j)) break;
+              outputs(t, t, vslot, j == 0);
+              if (t == 1) umma_commit(empty + vslot % SLOTS);
+              if (j + 1 < n) {
+                if (C::P_IN_S && !need(o_done + t, tn + j)) break;
+                scores(t, t, kslot);
+              }
+            }
+            if (ok && j + 1 < n) {
+              umma_commit(empty + kslot % SLOTS);
+              if (j + 2 == n) umma_commit(q_empty);
+            }
+          }
+        } else {
+          scores(0, tn & 1, kv);
+          umma_commit(empty + kv % SLOTS);
+          if (n == 1) umma_commit(q_empty);
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t vslot = kv + 2 * j + 1, kslot = vslot + 1, buf = (tn + j) & 1;
+            if (j + 1 < n) {
+              if (!need(full + kslot % SLOTS, kslot / SLOTS)) break;
+              scores(0, buf ^ 1, kslot);
+              umma_commit(empty + kslot % SLOTS);
+              if (j + 2 == n) umma_commit(q_empty);
+            }
+            if (!need(full + vslot % SLOTS, vslot / SLOTS) || !need(p_full + buf, (tn + j) >> 1)) break;
+            outputs(0, buf, vslot, j == 0);
+            umma_commit(empty + vslot % SLOTS);
+          }
+        }
+        kv += 2 * n;
+        tn += n;
+        ++qn;
+      }
+      if (!ok) {
+        give_up();
+        if (tn) mbar_wait_ns(o_done, (tn - 1) & 1, SSB_WAIT_NS);
+      }
+    }
+  } else if (warp >= PROD && warp < PROD + 4) {
+    const int pt = tid - PROD * 32, pw = pt >> 5;
+    Unit u;
+    uint32_t kv = 0, qn = 0;
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      const Range rg = range_for(u);
+      const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
+      const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
+      const int32_t* trow = a.table + (int64_t)max(u.row, 0) * a.max_pages;
+      if (qn && !mbar_wait_ns(q_empty, (qn - 1) & 1, SSB_WAIT_NS)) {
+        ok = false;
+        break;
+      }
+      ++qn;
+      for (int i = pt; i < C::MB * CPR; i += 128) {
+        const int r = i / CPR, c = i % CPR, f = u.r0 + r, t = f / a.group, g = f - t * a.group;
+        const bool in = r < u.rows;
+        const uint16_t* src = a.q + (in ? (u.q0 + (int64_t)t) * a.q_tok + (u.h * a.group + g) * a.q_head + c * 8 : 0);
+        cp_async16(smem_u32(sq) + (c >> 3) * (C::MB * 128) + swz128(r, c & 7), src, in ? 16 : 0);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      // tokens of this warp: rows [pw * T / 4, (pw + 1) * T / 4) of a tile; lane l holds the offset of row l
+      auto offset_of = [&](int i) -> long long {
+        if (i >= u.i1 || lane >= T / 4) return -1;
+        const int t = tile_token(rg, i, T) + pw * (T / 4) + lane;
+        if (!seen_by_any(a, t, p_lo, p_hi)) return -1;
+        const int j = page_of(a, t), page = trow[j];
+        if (page < 0 || page >= a.pages) {
+          set_err(a.err, SSB_ERR_PAGE_RANGE);
+          return -1;
+        }
+        return (long long)page * a.sp + (long long)(t - j * a.page_size) * a.st;
+      };
+      uint32_t first = kv;                            // oldest slot that is not handed over yet
+      bool q_given = false;
+      auto hand_over = [&](uint32_t upto) {           // the copies of the slots before `upto` have landed
+        fence_proxy_async_smem();
+        if (!q_given && first < upto) {
+          q_given = true;
+          mbar_arrive(q_full);
+        }
+        for (; first < upto; ++first) mbar_arrive(full + first % SLOTS);
+      };
+      long long off = offset_of(u.i0);
+      for (int i = u.i0; i < u.i1 && ok; ++i) {
+        const long long off_next = offset_of(i + 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ok && kv >= SLOTS && !mbar_wait_ns(empty + kv % SLOTS, (kv / SLOTS - 1) & 1, SSB_WAIT_NS)) ok = false;
+          if (!ok) break;
+          const uint32_t dst = smem_u32(ring + (kv % SLOTS) * C::SLOT);
+          const uint16_t* base = x ? vh : kh;
+          constexpr int RPP = 32 / CPR > 0 ? 32 / CPR : 1, PASSES = (T / 4) * CPR / 32;
+#pragma unroll
+          for (int v = 0; v < PASSES; ++v) {
+            const int r = v * RPP + lane / CPR, c = lane % CPR;
+            const long long o = __shfl_sync(0xFFFFFFFFu, off, r);
+            const uint32_t row = pw * (T / 4) + r;
+            cp_async16(dst + (c >> 3) * (T * 128) + swz128(row, c & 7), base + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          ++kv;
+          if (kv - first > LAG) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
+            hand_over(kv - LAG);
+          }
+        }
+        off = off_next;
+      }
+      cp_async_wait_all();
+      if (ok) hand_over(kv);
+    }
+    cp_async_wait_all();
+    if (!ok) give_up();
+  } else if (warp < PROD) {
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
+    Unit u;
+    uint32_t tn = 0;
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      const Range rg = range_for(u);
+      const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
+      const int pos = p + min(f0 + row, last) / a.group;       // rows past the last: zero queries, never written
+      const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
+      float m = -INFINITY, l = 0.f;
+      for (int i = u.i0; i < u.i1; ++i, ++tn) {
+        const int buf = NT == 2 ? t : tn & 1;
+        if (!warp_wait(s_full + buf, NT == 2 ? tn : tn >> 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * C::P_STEP;
+        const int tok = tile_token(rg, i, T);
+        const bool whole = seen_by_all(a, tok, tok + T, t_lo, t_hi);
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < T; c += 32) {
+          float v[32];
+          tmem_ld32(sc + c, v);
+          if (whole) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) mx = fmaxf(mx, v[x]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) mx = seen(a, tok + c + x, pos) ? fmaxf(mx, v[x]) : mx;
+          }
+        }
+        mx *= a.scale_log2;
+        if (i == u.i0) {
+          m = mx;
+        } else {
+          const bool up = mx > m + 8.f;
+          if (__any_sync(0xFFFFFFFFu, up)) {
+            if (!warp_wait(o_done + t, tn - 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const float f = up ? ex2(m - mx) : 1.f;
+            if (up) m = mx;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float v[32];
+              tmem_ld32(lane_base + t * D + c, v);
+              uint32_t r[32];
+#pragma unroll
+              for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(v[x] * f);
+              tmem_st16(lane_base + t * D + c, r);
+              tmem_st16(lane_base + t * D + c + 16, r + 16);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+        for (int c = 0; c < T; c += 32) {
+          float v[32];
+          tmem_ld32(sc + c, v);
+          if (!whole) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = seen(a, tok + c + x, pos) ? v[x] : -INFINITY;
+          }
+          uint32_t r[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float p0 = ex2(fmaf(v[2 * x], a.scale_log2, -mu)), p1 = ex2(fmaf(v[2 * x + 1], a.scale_log2, -mu));
+            l += p0 + p1;
+            r[x] = pack2<E>(p0, p1);
+          }
+          tmem_st16(pc + c / 2, r);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_full + buf);
+      }
+      // With one row tile the last S was ordered before the product but one: a warp that is ahead of the others may still
+      // be two phases ahead of o_done, which a single parity wait would not see.
+      if (ok && NT == 1 && tn >= 2) ok = warp_wait(o_done + t, tn - 2);
+      if (!ok || !warp_wait(o_done + t, tn - 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int fr = f0 + row;
+      const bool in = t * 128 + row < u.rows;
+      const int tk = fr / a.group, hg = fr - tk * a.group;
+      const int64_t orow = (u.q0 + (int64_t)tk) * a.heads + u.h * a.group + hg;
+      const int64_t prow = (int64_t)u.slot * C::MB + t * 128 + row;
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float v[32];
+        tmem_ld32(lane_base + t * D + c, v);
+        if (!in) continue;
+        if (u.slot < 0) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *(uint4*)(a.out + orow * D + c + 8 * x) =
+                make_uint4(pack2<E>(v[8 * x] * inv, v[8 * x + 1] * inv), pack2<E>(v[8 * x + 2] * inv, v[8 * x + 3] * inv),
+                           pack2<E>(v[8 * x + 4] * inv, v[8 * x + 5] * inv), pack2<E>(v[8 * x + 6] * inv, v[8 * x + 7] * inv));
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            *(float4*)(a.acc + prow * D + c + 4 * x) = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+        }
+      }
+      if (in) {
+        if (u.slot >= 0) a.ml[prow] = make_float2(m, l);
+        else if (a.lse) a.lse[orow] = (m + log2f(l)) * LN2;
+      }
+    }
+    if (!ok) give_up();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA) tmem_dealloc(tmem, 512);
+  if (tid == 0 && *failed) set_err(a.err, SSB_ERR_TIMEOUT);
+}
+
+// Sums the pieces of the items that were cut: grid (joints at most, MB / 8), eight rows a block, D / 4 threads a row.
+template <typename E, int D>
+__global__ void __launch_bounds__(2 * D) k_prefill_join(Args a, Work w) {
+  pdl_wait();
+  if ((int)blockIdx.x >= w.ctl[2]) return;
+  const Joint j = w.joints[blockIdx.x];
+  const int r = blockIdx.y * 8 + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
+  if (r >= j.rows) return;
+  const int64_t at = (int64_t)j.slot * Cfg<D>::MB + r;
+  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < j.pieces; ++i) m = fmaxf(m, a.ml[at + (int64_t)i * Cfg<D>::MB].x);
+  const float u = m == -INFINITY ? 0.f : m;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < j.pieces; ++i) {
+    const int64_t s = at + (int64_t)i * Cfg<D>::MB;
+    const float2 e = a.ml[s];
+    const float f = ex2(e.x - u);
+    const float4 x = *(const float4*)(a.acc + s * D + c * 4);
+    l += e.y * f;
+    o.x += x.x * f;
+    o.y += x.y * f;
+    o.z += x.z * f;
+    o.w += x.w * f;
+  }
+  const int fr = j.r0 + r, t = fr / a.group, g = fr - t * a.group;
+  const int64_t row = (j.q0 + (int64_t)t) * a.heads + j.h * a.group + g;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  *(uint2*)(a.out + row * D + c * 4) = make_uint2(pack2<E>(o.x * inv, o.y * inv), pack2<E>(o.z * inv, o.w * inv));
+  if (a.lse && c == 0) a.lse[row] = (m + log2f(l)) * LN2;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+struct Layout {
+  int64_t item0, ctl, units, joints, ml, acc, bytes;
+  int max_units, max_slots;
+};
+int64_t up(int64_t x) { return (x + 127) / 128 * 128; }
+Layout layout_of(int dim, int n, int64_t rows, int heads, int kv_heads) {
+  const int mb = dim == 256 ? 128 : 256, blocks = sm_count();
+  Layout l;
+  const int64_t items = (rows * (heads / kv_heads) / mb + n) * kv_heads;
+  l.max_slots = 4 * blocks;
+  l.max_units = (int)items;
+  l.item0 = 0;
+  l.ctl = up((int64_t)(n + 1) * 4);
+  l.units = l.ctl + 128;
+  l.joints = l.units + up((items + l.max_slots) * (int64_t)sizeof(Unit));
+  l.ml = l.joints + up(l.max_slots / 2 * (int64_t)sizeof(Joint));
+  l.acc = l.ml + up((int64_t)l.max_slots * mb * 8);
+  l.bytes = l.acc + (int64_t)l.max_slots * mb * dim * 4;
+  return l;
+}
+
+template <typename E, int D>
+int launch(Args& a, uint8_t* ws, const Layout& l, cudaStream_t stream) {
+  using C = Cfg<D>;
+  Work w;
+  w.item0 = (int*)(ws + l.item0);
+  w.ctl = (int*)(ws + l.ctl);
+  w.units = (Unit*)(ws + l.units);
+  w.joints = (Joint*)(ws + l.joints);
+  w.max_units = l.max_units;
+  w.max_slots = l.max_slots;
+  a.ml = (float2*)(ws + l.ml);
+  a.acc = (float*)(ws + l.acc);
+  auto kern = k_prefill<E, D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return (int)e;
+  }
+  ssb_note_smem("attn_prefill", kern, C::SMEM);
+  const int blocks = sm_count();
+  int rc = ssb_launch(k_prefill_plan<C::MB, C::T>, dim3(1), dim3(PLAN_T), 0, stream, false, a, w, blocks);
+  if (rc) return rc;
+  rc = ssb_launch(kern, dim3(blocks), dim3(C::THREADS), C::SMEM, stream, true, a, w);
+  if (rc) return rc;
+  return ssb_launch(k_prefill_join<E, D>, dim3(l.max_slots / 2, C::MB / 8), dim3(2 * D), 0, stream, true, a, w);
+}
+
+}  // namespace
+
+int64_t prefill_workspace(int dim, int n, int64_t rows, int heads, int kv_heads) {
+  return layout_of(dim, n, rows, heads, kv_heads).bytes;
+}
+
+int prefill_launch(Args& a, int dim, bool bf16, void* ws, void* stream) {
+  const Layout l = layout_of(dim, a.n, a.rows, a.heads, a.kv_heads);
+  uint8_t* p = (uint8_t*)ws;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (bf16)
+    return dim == 64 ? launch<__nv_bfloat16, 64>(a, p, l, st)
+                     : dim == 128 ? launch<__nv_bfloat16, 128>(a, p, l, st) : launch<__nv_bfloat16, 256>(a, p, l, st);
+  return dim == 64 ? launch<__half, 64>(a, p, l, st)
+                   : dim == 128 ? launch<__half, 128>(a, p, l, st) : launch<__half, 256>(a, p, l, st);
+}
+
+}  // namespace attn

@@ -91,7 +91,7 @@ SIGNATURES = {
     "ssb_kv_fork": [_P, _P, _P, _I32, _P],
     "ssb_kv_free": [_P, _P, _P, _P, _I32, _P],
     "ssb_kv_compact": [_P, _P],
-    "ssb_attn_workspace": [_I32, _I32, _I32, _I64, _I32, _P],
+    "ssb_attn_workspace": [_I32, _I32, _I64, _I32, _I32, _I32, _P],
     "ssb_attn_decode": [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
                         _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
     "ssb_attn_prefill": [_P, _I32, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32,

@@ -23,13 +23,13 @@ _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _WS = {}
 
 
-def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, prefill: bool = False) -> int:
+def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, kv_heads: int, prefill: bool = False) -> int:
     """Bytes of ``ws`` for ``n`` sequences with ``rows`` query tokens in all."""
-    key = (head_dim, n, rows, heads, prefill, torch.cuda.current_device())
+    key = (head_dim, n, rows, heads, kv_heads, prefill, torch.cuda.current_device())
     got = _WS.get(key)
     if got is None:
         b = ctypes.c_int64()
-        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, int(prefill), rows, heads, ctypes.byref(b)),
+        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, rows, heads, kv_heads, int(prefill), ctypes.byref(b)),
                    "attention workspace")
         if len(_WS) > 4096:
             _WS.clear()
@@ -37,7 +37,7 @@ def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, prefill: bool 
     return got
 
 
-def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse):
+def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out, lse):
     tag = _TYPES.get(q.dtype)
     if tag is None or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
         raise ValueError("q, k_pages and v_pages must all be bf16 or all fp16")
@@ -60,6 +60,8 @@ def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window
         raise ValueError(f"{n} sequences, but page_table has {rows} rows")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
+    if scale is not None and not 0 < scale < math.inf:
+        raise ValueError("scale must be positive and finite")
     if err is not None and (err.dtype != torch.int32 or err.numel() != 1):
         raise ValueError("err must be one int32")
     shape = q.shape
@@ -72,8 +74,8 @@ def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window
     return tag, ks, rows, out
 
 
-def _workspace(ws, dim, n, rows, heads, prefill, device):
-    need = workspace_bytes(dim, n, rows, heads, prefill)
+def _workspace(ws, dim, n, rows, heads, kv_heads, prefill, device):
+    need = workspace_bytes(dim, n, rows, heads, kv_heads, prefill)
     if ws is None:
         return torch.empty(need, dtype=torch.uint8, device=device), need
     if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
@@ -89,8 +91,9 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, out=None, *, lse=None,
     if q.dim() != 4 or q.stride(3) != 1:
         raise ValueError("q must be [n, q_len, heads, head_dim] with a contiguous head_dim")
     n, q_len, heads, dim = q.shape
-    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse)
-    ws, ws_bytes = _workspace(ws, dim, n, n * q_len, heads, False, q.device)
+    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out,
+                               lse)
+    ws, ws_bytes = _workspace(ws, dim, n, n * q_len, heads, k_pages.shape[1], False, q.device)
     p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
     rc = _lib.lib().ssb_attn_decode(
         p(q), tag, qs[0], qs[1], qs[2], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], n, q_len, heads, kp[1], dim, kp[2],
@@ -111,8 +114,9 @@ def attn_prefill(q, k_pages, v_pages, page_table, lengths, starts, out=None, *, 
         raise ValueError("starts must be a contiguous int32 vector of at least one element")
     total, heads, dim = q.shape
     n = starts.numel() - 1
-    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, err, out, lse)
-    ws, ws_bytes = _workspace(ws, dim, n, total, heads, True, q.device)
+    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out,
+                               lse)
+    ws, ws_bytes = _workspace(ws, dim, n, total, heads, k_pages.shape[1], True, q.device)
     p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
     rc = _lib.lib().ssb_attn_prefill(
         p(q), tag, qs[0], qs[1], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], total, p(starts), n, heads, kp[1], dim,

@@ -112,6 +112,28 @@ def test_prefill_page_sizes_and_ids(ps):
     _prefill([300, 50, 411], [40, 411], 4, 1, 128, ps, BF, ids=[1, 2])
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_rise_or_fall_along_the_cache(dim, falling):
+    """Keys growing (or shrinking) with the position: the running maximum rises by far more than one step, over and over
+    (or not at all after the first tile), in some rows and not in others."""
+    n, new, heads, kv = 1500, 200, 4, 2
+    k, v, table, lens, g = _cache([n], kv, dim, 16, BF)
+    ramp = torch.linspace(0, 12, n, device="cuda")
+    ramp = ramp.flip(0) if falling else ramp
+    for t in range(0, n, 16):
+        m = min(16, n - t)
+        k[int(table[0, t // 16]), :, :m] *= ramp[t:t + m, None].to(BF)
+    q = _q(g, new, heads, kv, dim, BF)
+    q[::3] *= 0.01
+    starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    lse = torch.empty(new, heads, device="cuda")
+    out = attn_prefill(q, k, v, table, lens, starts, lse=lse)
+    assert_attention(out, lse, attention(q, k, v, table, lens, [new]))
+    out = attn_decode(q[-3:][None], k, v, table, lens, lse=lse[None, -3:])
+    assert_attention(out[0], lse[-3:], attention(q[-3:], k, v, table, lens, [3]))
+
+
 def test_prefill_long_context_few_rows():
     _prefill([9001], [3], 4, 2, 128, 32, BF)
     _prefill([6000], [17], 16, 2, 256, 16, HF, 5000, 8)
@@ -162,7 +184,7 @@ def test_pages_behind_the_window_are_not_read():
 def test_results_repeat_and_a_batch_equals_itself_in_a_graph():
     k, v, table, lens, g = _cache([700, 30, 2000], 2, 128, 16, BF)
     q = _q(g, 3, 16, 2, 128, BF).unflatten(0, (3, 1))
-    ws = torch.empty(workspace_bytes(128, 3, 3, 16), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(workspace_bytes(128, 3, 3, 16, 2), dtype=torch.uint8, device="cuda")
     out, ref = torch.empty(q.shape, dtype=BF, device="cuda"), attn_decode(q, k, v, table, lens)
     graph = torch.cuda.CUDAGraph()
     attn_decode(q, k, v, table, lens, out, ws=ws)

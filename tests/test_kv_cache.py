@@ -31,6 +31,8 @@ def test_state_size():
     (dict(lengths=torch.zeros(2, dtype=torch.int32)), "lengths"),
     (dict(kw=dict(window=-1)), "negative"),
     (dict(kw=dict(sinks=-1)), "negative"),
+    (dict(kw=dict(scale=0.0)), "scale"),
+    (dict(kw=dict(scale=float("nan"))), "scale"),
     (dict(kw=dict(ids=torch.zeros(2, dtype=torch.int32))), "ids"),
     (dict(kw=dict(lse=torch.zeros(1, 1, 4, 1))), "lse"),
     (dict(kw=dict(out=torch.zeros(1, 1, 4, 32, dtype=torch.bfloat16))), "out"),
@@ -124,7 +126,7 @@ def _decode_args(**change):
     (dict(ps=0), _lib.SSB_EINVAL), (dict(pages=0), _lib.SSB_EINVAL), (dict(rows=0), _lib.SSB_EINVAL),
     (dict(mp=1 << 28), _lib.SSB_EINVAL), (dict(window=-1), _lib.SSB_EINVAL), (dict(sinks=-1), _lib.SSB_EINVAL),
     (dict(st=63), _lib.SSB_EINVAL), (dict(qh=4), _lib.SSB_EINVAL), (dict(k=72), _lib.SSB_EINVAL),
-    (dict(n=-1), _lib.SSB_EINVAL), (dict(n=0), _lib.SSB_OK), (dict(q_len=0), _lib.SSB_OK),
+    (dict(scale=-1.0), _lib.SSB_EINVAL), (dict(n=-1), _lib.SSB_EINVAL), (dict(n=0), _lib.SSB_OK), (dict(q_len=0), _lib.SSB_OK),
     (dict(q=None, ws_bytes=1 << 40), _lib.SSB_EINVAL), (dict(ws=None, ws_bytes=1 << 40), _lib.SSB_EINVAL)])
 def test_c_attention_refusals(change, want):
     assert _lib.lib().ssb_attn_decode(*_decode_args(**change)) == want
