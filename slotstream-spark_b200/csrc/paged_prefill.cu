@@ -14,9 +14,11 @@
 //
 // Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V rows through
 // cp.async (any page size; rows that no query sees become zeros) into 128-byte-swizzled tiles, and one that issues
-// the matrix instructions; one lane of another hands out units. The two products have different shapes or accumulators, so
-// nothing orders them but the waits here: P has columns of its own where TMEM has room (head sizes 64 and 256); at 128
-// it takes the place of S, and the next S is not started before the product that reads P has finished.
+// the matrix instructions; one lane of another hands out units. The two products differ in shape and accumulator, so
+// nothing orders them but the waits here: P has TMEM columns of its own, and a product's end is waited for before its P
+// or its sum is touched. S is read into registers once; when P is written, S is free, so the next S is started before
+// the product with this P, and the softmax of the next tile waits for one product only. T = 80 is the largest multiple of
+// 16 that leaves room for two accumulators, two S and two P of head size 128 in the 512 columns.
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
@@ -32,13 +34,13 @@ namespace {
 
 template <int D>
 struct Cfg {
-  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 256 ? 64 : 128, SLOTS = D == 64 ? 8 : 5;
+  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 256 ? 64 : 80;
+  static constexpr int SLOTS = D == 64 ? 12 : D == 128 ? 8 : 5;
   static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
   // TMEM columns: the accumulators, two buffers of S, two of P (two elements a column)
-  static constexpr bool P_IN_S = D == 128;
-  static constexpr int S_COL = NT * D, P_COL = P_IN_S ? S_COL : S_COL + 2 * T, P_STEP = P_IN_S ? T : T / 2;
-  static_assert((P_IN_S ? S_COL : P_COL) + (P_IN_S ? 2 * T : T) <= 512, "TMEM");
+  static constexpr int S_COL = NT * D, P_COL = S_COL + 2 * T;
+  static_assert(P_COL + T <= 512, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 3;
 
@@ -198,11 +200,40 @@ __global__ void __launch_bounds__(PLAN_T) k_prefill_plan(Args a, Work w, int blo
   }
 }
 
-// mbar_wait_ns by a whole warp that goes on to warp-wide TMEM instructions: the lanes may leave the wait one by one, and
-// the vote brings them together again.
-SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xFFFFFFFFu, mbar_wait_ns(bar, parity & 1, SSB_WAIT_NS));
+// Waits for phase `parity` of `bar`, polling without a suspend-time hint: the roles hand tiles to one another several
+// times per microsecond, and waking from a long suspension costs more than a product. False after SSB_WAIT_NS.
+SSB_DEV bool wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity & 1)
+        : "memory");
+    if (done) return true;
+    if ((i & 255u) == 255u) {
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > SSB_WAIT_NS) return false;
+    }
+  }
 }
+SSB_DEV bool ready(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity & 1)
+      : "memory");
+  return done;
+}
+// The same by a whole warp that goes on to warp-wide TMEM instructions: the lanes may leave the wait one by one, and the
+// vote brings them together again.
+SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
 
 // D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column.
 SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
@@ -241,6 +272,36 @@ SSB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+SSB_DEV void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+SSB_DEV void tmem_ld16(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr));
+}
+// N columns of this thread's TMEM lane, all loads in flight together. The empty statements keep uses behind the wait.
+template <int N>
+SSB_DEV void tmem_ld_row(uint32_t taddr, float* v) {
+#pragma unroll
+  for (int c = 0; c < N; c += 16) tmem_ld16(taddr + c, v + c);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < N; c += 8)
+    asm volatile("" : "+f"(v[c]), "+f"(v[c + 1]), "+f"(v[c + 2]), "+f"(v[c + 3]), "+f"(v[c + 4]), "+f"(v[c + 5]), "+f"(v[c + 6]),
+                 "+f"(v[c + 7]));
+}
+// Bit x: token t0 + x (x < 32) is visible to the query at position p.
+SSB_DEV uint32_t bits_below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+SSB_DEV uint32_t seen_bits(const Args& a, int p, int t0) {
+  uint32_t m = bits_below(p + 1 - t0);
+  if (a.window) m &= ~bits_below(p - a.window + 1 - t0) | bits_below(a.sinks - t0);
+  return m;
 }
 SSB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -292,7 +353,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
   // The next unit, or false at the end of the list (or when a wait gave up).
   auto next_unit = [&](Unit& u) {
     const int s = un & 1;
-    if (!mbar_wait_ns(u_full + s, (un >> 1) & 1, SSB_WAIT_NS)) {
+    if (!wait(u_full + s, (un >> 1) & 1)) {
       give_up();
       return false;
     }
@@ -313,7 +374,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
       const int units = w.ctl[1];
       for (int k = 0;; ++k) {
         const int s = k & 1;
-        if (k >= 2 && !mbar_wait_ns(u_empty + s, ((k >> 1) - 1) & 1, SSB_WAIT_NS)) {
+        if (k >= 2 && !wait(u_empty + s, ((k >> 1) - 1) & 1)) {
           give_up();
           break;
         }
@@ -341,11 +402,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         const uint32_t vs = smem_u32(ring + (slot % SLOTS) * C::SLOT);
 #pragma unroll
         for (int k = 0; k < T / 16; ++k)
-          umma_ts(tmem + t * D, tmem + C::P_COL + buf * C::P_STEP + k * 8, umma_desc_mn(vs + k * 2048, T * 128), ID_O, !first || k > 0);
+          umma_ts(tmem + t * D, tmem + C::P_COL + buf * (T / 2) + k * 8, umma_desc_mn(vs + k * 2048, T * 128), ID_O, !first || k > 0);
         umma_commit(o_done + t);
       };
       auto need = [&](uint64_t* b, uint32_t parity) {
-        if (ok && !mbar_wait_ns(b, parity & 1, SSB_WAIT_NS)) ok = false;
+        if (ok && !wait(b, parity & 1)) ok = false;
         if (ok) tc_fence_after();
         return ok;
       };
@@ -353,28 +414,26 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         const int n = u.i1 - u.i0;
         if (!need(q_full, qn) || !need(full + kv % SLOTS, kv / SLOTS)) break;
         if constexpr (NT == 2) {
-          if (C::P_IN_S && tn && (!need(o_done, tn - 1) || !need(o_done + 1, tn - 1))) break;
           scores(0, 0, kv);
           scores(1, 1, kv);
           umma_commit(empty + kv % SLOTS);
           if (n == 1) umma_commit(q_empty);
           for (int j = 0; j < n && ok; ++j) {
             const uint32_t vslot = kv + 2 * j + 1, kslot = vslot + 1;
-            if (!need(full + vslot % SLOTS, vslot / SLOTS)) break;
-            if (j + 1 < n && !need(full + kslot % SLOTS, kslot / SLOTS)) break;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              if (!need(p_full + t, tn + j)) break;
+              if (!need(p_full + t, tn + j)) break;   // S has been read, P is there: the next S first, then the product
+              if (j + 1 < n) {
+                if (t == 0 && !need(full + kslot % SLOTS, kslot / SLOTS)) break;
+                scores(t, t, kslot);
+                if (t == 1) {
+                  umma_commit(empty + kslot % SLOTS);
+                  if (j + 2 == n) umma_commit(q_empty);
+                }
+              }
+              if (t == 0 && !need(full + vslot % SLOTS, vslot / SLOTS)) break;
               outputs(t, t, vslot, j == 0);
               if (t == 1) umma_commit(empty + vslot % SLOTS);
-              if (j + 1 < n) {
-                if (C::P_IN_S && !need(o_done + t, tn + j)) break;
-                scores(t, t, kslot);
-              }
-            }
-            if (ok && j + 1 < n) {
-              umma_commit(empty + kslot % SLOTS);
-              if (j + 2 == n) umma_commit(q_empty);
             }
           }
         } else {
@@ -400,7 +459,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
       }
       if (!ok) {
         give_up();
-        if (tn) mbar_wait_ns(o_done, (tn - 1) & 1, SSB_WAIT_NS);
+        if (tn) wait(o_done, (tn - 1) & 1);
       }
     }
   } else if (warp >= PROD && warp < PROD + 4) {
@@ -413,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
       const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
       const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
       const int32_t* trow = a.table + (int64_t)max(u.row, 0) * a.max_pages;
-      if (qn && !mbar_wait_ns(q_empty, (qn - 1) & 1, SSB_WAIT_NS)) {
+      if (qn && !wait(q_empty, (qn - 1) & 1)) {
         ok = false;
         break;
       }
@@ -452,7 +511,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         const long long off_next = offset_of(i + 1);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (ok && kv >= SLOTS && !mbar_wait_ns(empty + kv % SLOTS, (kv / SLOTS - 1) & 1, SSB_WAIT_NS)) ok = false;
+          if (kv >= SLOTS && !ready(empty + kv % SLOTS, kv / SLOTS - 1)) {
+            cp_async_wait_all();                       // nothing to issue: hand over what is on its way first
+            hand_over(kv);
+            ok = wait(empty + kv % SLOTS, kv / SLOTS - 1);
+          }
           if (!ok) break;
           const uint32_t dst = smem_u32(ring + (kv % SLOTS) * C::SLOT);
           const uint16_t* base = x ? vh : kh;
@@ -497,74 +560,83 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
           break;
         }
         tc_fence_after();
-        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * C::P_STEP;
+        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * (T / 2);
         const int tok = tile_token(rg, i, T);
-        const bool whole = seen_by_all(a, tok, tok + T, t_lo, t_hi);
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < T; c += 32) {
-          float v[32];
-          tmem_ld32(sc + c, v);
-          if (whole) {
+        float v[T];
+        tmem_ld_row<T>(sc, v);
+        if (!seen_by_all(a, tok, tok + T, t_lo, t_hi)) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) mx = fmaxf(mx, v[x]);
-          } else {
+          for (int c = 0; c < T; c += 16) {
+            const uint32_t bits = seen_bits(a, pos, tok + c);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) mx = seen(a, tok + c + x, pos) ? fmaxf(mx, v[x]) : mx;
+            for (int x = 0; x < 16; ++x)
+              if (!(bits >> x & 1)) v[c + x] = -INFINITY;
           }
         }
-        mx *= a.scale_log2;
+        float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int x = 4; x < T; x += 8) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            m4[y] = x + 4 + y < T ? fmaxf(m4[y], fmaxf(v[x + y], v[x + 4 + y])) : fmaxf(m4[y], v[x + y]);
+        }
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+        bool pending = i > u.i0;
         if (i == u.i0) {
           m = mx;
         } else {
-          const bool up = mx > m + 8.f;
-          if (__any_sync(0xFFFFFFFFu, up)) {
+          // The product of the tile before reads the P that is written next (with one row tile: the other buffer) and adds to
+          // the sum that may be rescaled. A parity wait sees one phase back only, so it is waited for at every tile.
+          const bool raise = mx > m + 8.f, any = __any_sync(0xFFFFFFFFu, raise);
+          if (NT == 2 || any) {
             if (!warp_wait(o_done + t, tn - 1)) {
               ok = false;
               break;
             }
+            pending = false;
+          }
+          if (any) {
             tc_fence_after();
-            const float f = up ? ex2(m - mx) : 1.f;
-            if (up) m = mx;
+            const float f = raise ? ex2(m - mx) : 1.f;
+            if (raise) m = mx;
             l *= f;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              float v[32];
-              tmem_ld32(lane_base + t * D + c, v);
-              uint32_t r[32];
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_ld_row<16>(lane_base + t * D + c, o);
+              uint32_t r[16];
 #pragma unroll
-              for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(v[x] * f);
+              for (int x = 0; x < 16; ++x) r[x] = __float_as_uint(o[x] * f);
               tmem_st16(lane_base + t * D + c, r);
-              tmem_st16(lane_base + t * D + c + 16, r + 16);
             }
-            tmem_st_wait();
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int c = 0; c < T; c += 32) {
-          float v[32];
-          tmem_ld32(sc + c, v);
-          if (!whole) {
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), mu2 = make_float2(-mu, -mu);
+        float2 l2 = make_float2(0.f, 0.f), l3 = l2;
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = seen(a, tok + c + x, pos) ? v[x] : -INFINITY;
-          }
-          uint32_t r[16];
+        for (int c = 0; c < T; c += 16) {
+          uint32_t r[8];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float p0 = ex2(fmaf(v[2 * x], a.scale_log2, -mu)), p1 = ex2(fmaf(v[2 * x + 1], a.scale_log2, -mu));
-            l += p0 + p1;
-            r[x] = pack2<E>(p0, p1);
+          for (int x = 0; x < 8; ++x) {
+            float2 e = __ffma2_rn(make_float2(v[c + 2 * x], v[c + 2 * x + 1]), sc2, mu2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            if (x & 1) l3 = __fadd2_rn(l3, e);
+            else l2 = __fadd2_rn(l2, e);
+            r[x] = pack2<E>(e.x, e.y);
           }
-          tmem_st16(pc + c / 2, r);
+          tmem_st8(pc + c / 2, r);
         }
+        l += (l2.x + l2.y) + (l3.x + l3.y);
         tmem_st_wait();
+        if (NT == 1 && pending && !warp_wait(o_done + t, tn - 1)) {
+          ok = false;
+          break;
+        }
         tc_fence_before();
         mbar_arrive(p_full + buf);
       }
-      // With one row tile the last S was ordered before the product but one: a warp that is ahead of the others may still
-      // be two phases ahead of o_done, which a single parity wait would not see.
-      if (ok && NT == 1 && tn >= 2) ok = warp_wait(o_done + t, tn - 2);
       if (!ok || !warp_wait(o_done + t, tn - 1)) {
         ok = false;
         break;
@@ -579,7 +651,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float v[32];
-        tmem_ld32(lane_base + t * D + c, v);
+        tmem_ld_row<32>(lane_base + t * D + c, v);
         if (!in) continue;
         if (u.slot < 0) {
 #pragma unroll
