@@ -435,6 +435,14 @@ int launch_dim(Args& a, int dim, uint8_t* ws, cudaStream_t st) {
   return launch_rows<E, 256>(a, ws, st);
 }
 
+// t / d = (mulhi(t, mul) + t) >> shift for t < 2^31 (round-up reciprocal of a 32-bit division).
+void reciprocal(int32_t d, uint32_t* mul, uint32_t* shift) {
+  uint32_t s = 0;
+  while ((1ull << s) < (uint64_t)d) ++s;
+  *shift = s;
+  *mul = (uint32_t)(((1ull << 32) * ((1ull << s) - (uint64_t)d)) / (uint64_t)d + 1);
+}
+
 // Checks and the fields that both entry points share.
 int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, int64_t page_stride,
          int64_t head_stride, int64_t token_stride, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim,
@@ -471,11 +479,8 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
   a.out = (uint16_t*)out;
   a.lse = lse;
   a.err = err;
-  // t / page_size = (mulhi(t, mul) + t) >> shift for t < 2^31 (round-up reciprocal of a 32-bit division)
-  uint32_t sh = 0;
-  while ((1ull << sh) < (uint64_t)page_size) ++sh;
-  a.page_shift = sh;
-  a.page_mul = (uint32_t)(((1ull << 32) * ((1ull << sh) - (uint64_t)page_size)) / (uint64_t)page_size + 1);
+  reciprocal(page_size, &a.page_mul, &a.page_shift);
+  reciprocal(a.group, &a.group_mul, &a.group_shift);
   return SSB_OK;
 }
 

@@ -21,7 +21,8 @@ struct Args {
   const int32_t* starts;              // ragged rows; nullptr: q_len rows of every sequence
   int32_t n, q_len, heads, kv_heads, group;
   int32_t page_size, pages, table_rows, max_pages;
-  uint32_t page_mul, page_shift;      // t / page_size for t < 2^31
+  uint32_t page_mul, page_shift;      // t / page_size for t < 2^31: (mulhi(t, mul) + t) >> shift
+  uint32_t group_mul, group_shift;    // the same for the group
   const int32_t *table, *lengths, *ids;
   int32_t window, sinks;
   float scale_log2;                   // scale * log2(e)

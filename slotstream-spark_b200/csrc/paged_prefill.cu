@@ -13,12 +13,13 @@
 // both types and the fp32 sums hold with the same relative precision, and rescaling the accumulator in TMEM becomes rare.
 //
 // Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V rows through
-// cp.async (any page size; rows that no query sees become zeros) into 128-byte-swizzled tiles, and one that issues
-// the matrix instructions; one lane of another hands out units. The two products differ in shape and accumulator, so
-// nothing orders them but the waits here: P has TMEM columns of its own, and a product's end is waited for before its P
-// or its sum is touched. S is read into registers once; when P is written, S is free, so the next S is started before
-// the product with this P, and the softmax of the next tile waits for one product only. T = 80 is the largest multiple of
-// 16 that leaves room for two accumulators, two S and two P of head size 128 in the 512 columns.
+// cp.async (any page size; rows that no query sees become zeros) into 128-byte-swizzled tiles and hand out the units, and one
+// per row tile and product that issues its matrix instructions. Nothing orders products of different threads, shapes or
+// accumulators but the waits here. S is read into registers once. At sizes 64 and 256 tiles are 64 tokens, P has TMEM
+// columns of its own, and S is free as soon as it has been read: the next S runs under the exponentials. At 128 the
+// accumulators and two S of 128 tokens fill TMEM; P takes the place of S, the next S waits for the product that reads P, and
+// that product starts with the first half of P. (Shorter tiles cost the tensor cores more there: an instruction of 64 or 80
+// columns takes 48 or 54 cycles, bound by reading its operands from shared memory, one of 128 takes 64.)
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
@@ -34,15 +35,19 @@ namespace {
 
 template <int D>
 struct Cfg {
-  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 256 ? 64 : 80;
-  static constexpr int SLOTS = D == 64 ? 12 : D == 128 ? 8 : 5;
+  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 128 ? 128 : 64, SLOTS = D == 64 ? 16 : 5;
   static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
-  // TMEM columns: the accumulators, two buffers of S, two of P (two elements a column)
-  static constexpr int S_COL = NT * D, P_COL = S_COL + 2 * T;
-  static_assert(P_COL + T <= 512, "TMEM");
+  // TMEM columns: the accumulators, two buffers of S, two of P (two elements a column; in the place of S at size 128)
+  static constexpr bool P_IN_S = D == 128;
+  static constexpr int S_COL = NT * D, P_COL = P_IN_S ? S_COL : S_COL + 2 * T, P_STEP = P_IN_S ? T : T / 2;
+  static_assert(S_COL + 2 * T <= 512 && P_COL + P_STEP + T / 2 <= 512, "TMEM");
+  // With 128 columns of S in a softmax thread's registers, the softmax warps take some from the others:
+  // 256 x R_SOFT + 256 x R_REST = 512 x R_LAUNCH.
+  static constexpr int R_SOFT = 192, R_REST = 64, R_LAUNCH = 128;
+  static_assert(!P_IN_S || 256 * R_SOFT + 256 * R_REST == THREADS * R_LAUNCH, "registers");
 };
-constexpr int PLAN_T = 1024, LAG = 3;
+constexpr int PLAN_T = 1024, LAG = 1;
 
 struct __align__(16) Unit {
   int b, h, r0, rows;          // sequence, key head, first flat row, rows
@@ -53,12 +58,19 @@ struct __align__(16) Joint {
   int h, r0, rows, q0, slot, pieces, pad0, pad1;
 };
 
+// Tensor maps of a call: q [rows, heads, dim] in boxes of 128 flat rows x 64, k and v [pages, kv_heads, page, dim] in boxes of
+// page_rows tokens x 64.
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
 struct Work {
   int* item0;                  // [n + 1] first item of each sequence
   int* ctl;                    // [0] units taken, [1] units, [2] joints
   Unit* units;
   Joint* joints;
   int max_units, max_slots;
+  int page_rows, q_boxes;      // tokens of a K / V box, 0: by cp.async; whether Q comes in boxes
 };
 
 SSB_DEV int block_scan(int v, int* part, int* total) {
@@ -200,27 +212,6 @@ __global__ void __launch_bounds__(PLAN_T) k_prefill_plan(Args a, Work w, int blo
   }
 }
 
-// Waits for phase `parity` of `bar`, polling without a suspend-time hint: the roles hand tiles to one another several
-// times per microsecond, and waking from a long suspension costs more than a product. False after SSB_WAIT_NS.
-SSB_DEV bool wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  uint64_t t0 = 0;
-  for (uint32_t i = 0;; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(addr), "r"(parity & 1)
-        : "memory");
-    if (done) return true;
-    if ((i & 255u) == 255u) {
-      const uint64_t t = globaltimer_ns();
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > SSB_WAIT_NS) return false;
-    }
-  }
-}
 SSB_DEV bool ready(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -231,28 +222,71 @@ SSB_DEV bool ready(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done;
 }
+// Waits for phase `parity`; false after SSB_WAIT_NS. try_wait: a waiting thread sleeps instead of taking issue slots from the
+// softmax; no suspend-time hint: the roles hand tiles to one another several times per microsecond.
+SSB_DEV bool wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  uint32_t i = 0;
+#pragma unroll 1
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity & 1)
+        : "memory");
+    if (done) return true;
+    if (++i & 63u) continue;                         // the global timer is slow to read
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    else if (t - t0 > SSB_WAIT_NS) return false;
+  }
+}
 // The same by a whole warp that goes on to warp-wide TMEM instructions: the lanes may leave the wait one by one, and the
 // vote brings them together again.
 SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
 
-// D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column.
-SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory descriptors as (low word, constant high word): moving inside a tile adds to the low word only. That keeps
+// the one thread that issues the products off the critical path -- with descriptors built from scratch it took about 100
+// cycles an instruction, more than the instruction itself.
+SSB_DEV uint32_t desc_lo(uint32_t smem_addr, uint32_t lead) { return (smem_addr >> 4) | (lead >> 4) << 16; }
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;     // 1024 bytes between groups of 8 rows, 128-byte swizzle
+// K-major tile (rows of 64 elements of the summed index); `lead` is not used by the swizzled form.
+constexpr uint32_t LEAD_K = 16;
+
+// One box of a 3-D / 4-D tensor map; the bytes are counted on `bar`.
+SSB_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-// Descriptor of a tile whose rows are the K index (tokens) and whose 128-byte swizzled panels hold 64 of the N index:
-// panels `panel` bytes apart, groups of eight tokens 1024 bytes apart.
-SSB_DEV uint64_t umma_desc_mn(uint32_t smem_addr, uint32_t panel) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(panel >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
+SSB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T.
+SSB_DEV void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column. B's rows are the
+// summed index (tokens); its 128-byte panels hold 64 of the N index and lie the descriptor's lead apart.
+SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      : "memory");
 }
 template <typename E>
 __host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn);
@@ -306,15 +340,15 @@ SSB_DEV uint32_t seen_bits(const Args& a, int p, int t0) {
 SSB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename E, int D>
-__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) {
+__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_constant__ Maps maps, Args a, Work w) {
   using C = Cfg<D>;
   constexpr int NT = C::NT, T = C::T, CPR = C::CPR, SLOTS = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
   uint8_t* ring = smem + C::QB;
   uint64_t* bar = (uint64_t*)(ring + SLOTS * C::SLOT);
-  uint64_t *q_full = bar, *q_empty = bar + 1, *s_full = bar + 2, *p_full = bar + 4, *o_done = bar + 6, *u_full = bar + 8,
-           *u_empty = bar + 10, *full = bar + 12, *empty = full + SLOTS;
+  uint64_t *q_full = bar, *q_empty = bar + 1, *s_full = bar + 2, *s_free = bar + 4, *p_full = bar + 6, *o_done = bar + 8,
+           *u_full = bar + 10, *u_empty = bar + 12, *drained = bar + 14, *p_half = bar + 18, *turn = bar + 20, *full = bar + 22, *empty = full + SLOTS;
   int* u_slot = (int*)(empty + SLOTS);             // unit numbers handed out, two in flight
   uint32_t* tmem_slot = (uint32_t*)(u_slot + 2);
   int* failed = (int*)(tmem_slot + 1);
@@ -323,22 +357,26 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
     if (tid == 0) set_err(a.err, SSB_ERR_MISALIGNED);
     return;
   }
-  constexpr int PROD = NT * 4, MMA = PROD + 4, SCHED = MMA + 1;      // first warps of the roles
+  constexpr int PROD = NT * 4, MMA = PROD + 4;    // first warps of the roles
 
   if (warp == MMA) tmem_alloc(tmem_slot, 512);
   if (tid == 0) {
     mbar_init(q_full, 128);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, NT);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 128);
       mbar_init(p_full + i, 128);
+      mbar_init(p_half + i, 128);
+      mbar_init(turn + i, 128);
       mbar_init(o_done + i, 1);
       mbar_init(u_full + i, 1);
-      mbar_init(u_empty + i, NT * 128 + 128 + 1);
+      mbar_init(u_empty + i, NT * 128 + 128 + 2 * NT);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(drained + i, 1);
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(full + i, 128);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, NT);
     }
     *failed = 0;
     fence_mbar_init();
@@ -369,105 +407,98 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
     return range_of(a, p + u.r0 / a.group, p + (u.r0 + u.rows - 1) / a.group, T);
   };
 
-  if (warp == SCHED) {
-    if (lane == 0) {
-      const int units = w.ctl[1];
-      for (int k = 0;; ++k) {
-        const int s = k & 1;
-        if (k >= 2 && !wait(u_empty + s, ((k >> 1) - 1) & 1)) {
-          give_up();
-          break;
-        }
-        const int i = *(volatile int*)failed ? units : atomicAdd(w.ctl, 1);
-        *(volatile int*)(u_slot + s) = i < units ? i : -1;
-        mbar_arrive(u_full + s);
-        if (i >= units) break;
-      }
-    }
-  } else if (warp == MMA) {
-    if (lane == 0) {
-      constexpr uint32_t ID_S = idesc_of<E>(128, T, false), ID_O = idesc_of<E>(128, D, true);
-      Unit u;
-      uint32_t kv = 0, qn = 0, tn = 0;              // slots, units and tiles so far
-      bool ok = true;
-      auto scores = [&](int t, int buf, uint32_t slot) {
-        const uint32_t ks = smem_u32(ring + (slot % SLOTS) * C::SLOT), qs = smem_u32(sq);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_bf16(tmem + C::S_COL + buf * T, umma_desc_sw128(qs + (k / 4) * (C::MB * 128) + t * 128 * 128 + (k % 4) * 32),
-                    umma_desc_sw128(ks + (k / 4) * (T * 128) + (k % 4) * 32), ID_S, k > 0);
-        umma_commit(s_full + buf);
-      };
-      auto outputs = [&](int t, int buf, uint32_t slot, bool first) {
-        const uint32_t vs = smem_u32(ring + (slot % SLOTS) * C::SLOT);
-#pragma unroll
-        for (int k = 0; k < T / 16; ++k)
-          umma_ts(tmem + t * D, tmem + C::P_COL + buf * (T / 2) + k * 8, umma_desc_mn(vs + k * 2048, T * 128), ID_O, !first || k > 0);
-        umma_commit(o_done + t);
-      };
-      auto need = [&](uint64_t* b, uint32_t parity) {
-        if (ok && !wait(b, parity & 1)) ok = false;
-        if (ok) tc_fence_after();
-        return ok;
-      };
-      while (ok && next_unit(u)) {
-        const int n = u.i1 - u.i0;
-        if (!need(q_full, qn) || !need(full + kv % SLOTS, kv / SLOTS)) break;
-        if constexpr (NT == 2) {
-          scores(0, 0, kv);
-          scores(1, 1, kv);
-          umma_commit(empty + kv % SLOTS);
-          if (n == 1) umma_commit(q_empty);
-          for (int j = 0; j < n && ok; ++j) {
-            const uint32_t vslot = kv + 2 * j + 1, kslot = vslot + 1;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!need(p_full + t, tn + j)) break;   // S has been read, P is there: the next S first, then the product
-              if (j + 1 < n) {
-                if (t == 0 && !need(full + kslot % SLOTS, kslot / SLOTS)) break;
-                scores(t, t, kslot);
-                if (t == 1) {
-                  umma_commit(empty + kslot % SLOTS);
-                  if (j + 2 == n) umma_commit(q_empty);
-                }
-              }
-              if (t == 0 && !need(full + vslot % SLOTS, vslot / SLOTS)) break;
-              outputs(t, t, vslot, j == 0);
-              if (t == 1) umma_commit(empty + vslot % SLOTS);
-            }
+  auto few_registers = [] {
+    if constexpr (C::P_IN_S) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
+  };
+  if (warp >= MMA) {
+   few_registers();
+   if (warp < MMA + 2 * NT && lane == 0) {
+    // One warp per row tile and product: a thread that waits on a barrier between two products leaves the tensor cores
+    // idle for about 170 cycles (its queue is short), unless another thread's products fill the gap.
+    constexpr uint32_t ID_S = idesc_of<E>(128, T, false), ID_O = idesc_of<E>(128, D, true);
+    const int t = (warp - MMA) % NT;
+    const bool scores = warp < MMA + NT;
+    const uint32_t q_lo = desc_lo(smem_u32(sq) + t * 128 * 128, LEAD_K), k_lo = desc_lo(smem_u32(ring), LEAD_K),
+                   v_lo = desc_lo(smem_u32(ring), T * 128);
+    Unit u;
+    uint32_t kv = 0, qn = 0, tn = 0;                // slots, units and tiles so far
+    bool ok = true;
+    auto need = [&](uint64_t* b, uint32_t parity) { ok = ok && wait(b, parity); };
+    while (ok && next_unit(u)) {
+      if (scores) need(q_full, qn++);
+#pragma unroll 1
+      for (int i = u.i0; i < u.i1 && ok; ++i, ++tn, kv += 2) {
+        const uint32_t buf = NT == 2 ? t : tn & 1, use = NT == 2 ? tn : tn >> 1;
+        if (scores) {
+          const uint32_t slot = kv % SLOTS;
+          need(full + slot, kv / SLOTS);
+          // what is in this buffer has been read: S by the softmax, or the P in its place by the product before
+          if (C::P_IN_S) {
+            if (tn) need(o_done + t, tn - 1);
+          } else if (use) {
+            need(s_free + buf, use - 1);
           }
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t kd = k_lo + slot * (C::SLOT >> 4), sd = tmem + C::S_COL + buf * T;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), kd + (((k / 4) * (T * 128) + (k % 4) * 32) >> 4),
+                    ID_S, k > 0);
+          umma_commit(s_full + buf);
+          umma_commit(empty + slot);
         } else {
-          scores(0, tn & 1, kv);
-          umma_commit(empty + kv % SLOTS);
-          if (n == 1) umma_commit(q_empty);
-          for (int j = 0; j < n && ok; ++j) {
-            const uint32_t vslot = kv + 2 * j + 1, kslot = vslot + 1, buf = (tn + j) & 1;
-            if (j + 1 < n) {
-              if (!need(full + kslot % SLOTS, kslot / SLOTS)) break;
-              scores(0, buf ^ 1, kslot);
-              umma_commit(empty + kslot % SLOTS);
-              if (j + 2 == n) umma_commit(q_empty);
-            }
-            if (!need(full + vslot % SLOTS, vslot / SLOTS) || !need(p_full + buf, (tn + j) >> 1)) break;
-            outputs(0, buf, vslot, j == 0);
-            umma_commit(empty + vslot % SLOTS);
+          const uint32_t slot = (kv + 1) % SLOTS;
+          need(full + slot, (kv + 1) / SLOTS);
+          const uint32_t vd = v_lo + slot * (C::SLOT >> 4), pd = tmem + C::P_COL + buf * C::P_STEP, od = tmem + t * D;
+          constexpr int HALF = C::P_IN_S ? T / 32 : 0;   // k steps that can start with the first half of P
+          if constexpr (HALF > 0) {
+            need(p_half + buf, use);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < HALF; ++k) umma_ts(od, pd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
           }
+          need(p_full + buf, use);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = HALF; k < T / 16; ++k) umma_ts(od, pd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
+          umma_commit(o_done + t);
+          umma_commit(empty + slot);
         }
-        kv += 2 * n;
-        tn += n;
-        ++qn;
       }
-      if (!ok) {
-        give_up();
-        if (tn) wait(o_done, (tn - 1) & 1);
-      }
+      if (scores && ok) umma_commit(q_empty);
     }
-  } else if (warp >= PROD && warp < PROD + 4) {
+    if (!ok) give_up();
+    umma_commit(drained + (warp - MMA));            // nothing of this thread's may run when TMEM goes
+    if (!wait(drained + (warp - MMA), 0)) give_up();
+   }
+  } else if (warp >= PROD) {
+    few_registers();
     const int pt = tid - PROD * 32, pw = pt >> 5;
     Unit u;
     uint32_t kv = 0, qn = 0;
     bool ok = true;
+    // The first of these threads also hands out the units, one ahead of its own use.
+    const int units = w.ctl[1];
+    uint32_t given = 0;
+    auto give_unit = [&] {
+      if (pt) return true;
+      const uint32_t slot = given & 1;
+      if (given >= 2 && !wait(u_empty + slot, (given >> 1) - 1)) return false;
+      const int i = atomicAdd(w.ctl, 1);
+      *(volatile int*)(u_slot + slot) = i < units ? i : -1;
+      mbar_arrive(u_full + slot);
+      ++given;
+      return true;
+    };
+    ok = give_unit();
     while (ok && next_unit(u)) {
+      if (!give_unit()) {
+        ok = false;
+        break;
+      }
       const Range rg = range_for(u);
       const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
       const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
@@ -477,13 +508,30 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         break;
       }
       ++qn;
-      for (int i = pt; i < C::MB * CPR; i += 128) {
-        const int r = i / CPR, c = i % CPR, f = u.r0 + r, t = f / a.group, g = f - t * a.group;
-        const bool in = r < u.rows;
-        const uint16_t* src = a.q + (in ? (u.q0 + (int64_t)t) * a.q_tok + (u.h * a.group + g) * a.q_head + c * 8 : 0);
-        cp_async16(smem_u32(sq) + (c >> 3) * (C::MB * 128) + swz128(r, c & 7), src, in ? 16 : 0);
+      const bool boxes = w.q_boxes != 0;
+      if (boxes) {
+        constexpr int N = NT * (D / 64);               // one box per row tile and 64 columns
+        if (pt < N) {
+          const int t = pt % NT, c = pt / NT;
+          mbar_expect_tx(q_full, 128 * 128);
+          tma_load_3d(smem_u32(sq) + c * (C::MB * 128) + t * (128 * 128), &maps.q, c * 64, u.h * a.group,
+                      u.q0 + (u.r0 + t * 128) / a.group, q_full);
+        } else {
+          mbar_arrive(q_full);
+        }
+      } else {
+        constexpr int RPP = 128 / CPR;                 // rows a pass
+        const int c = pt % CPR;
+        const uint32_t dst = smem_u32(sq) + (c >> 3) * (C::MB * 128);
+        const uint16_t* base = a.q + (int64_t)u.q0 * a.q_tok + (int64_t)u.h * a.group * a.q_head + c * 8;
+#pragma unroll 4
+        for (int r = pt / CPR; r < C::MB; r += RPP) {
+          const int f = u.r0 + r, t = (int)((__umulhi((uint32_t)f, a.group_mul) + (uint32_t)f) >> a.group_shift);
+          const int64_t off = t * a.q_tok + (f - t * a.group) * a.q_head;
+          cp_async16(dst + swz128(r, c & 7), base + (r < u.rows ? off : 0), r < u.rows ? 16 : 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
       // tokens of this warp: rows [pw * T / 4, (pw + 1) * T / 4) of a tile; lane l holds the offset of row l
       auto offset_of = [&](int i) -> long long {
         if (i >= u.i1 || lane >= T / 4) return -1;
@@ -497,7 +545,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         return (long long)page * a.sp + (long long)(t - j * a.page_size) * a.st;
       };
       uint32_t first = kv;                            // oldest slot that is not handed over yet
-      bool q_given = false;
+      bool q_given = boxes;
       auto hand_over = [&](uint32_t upto) {           // the copies of the slots before `upto` have landed
         fence_proxy_async_smem();
         if (!q_given && first < upto) {
@@ -506,47 +554,100 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         }
         for (; first < upto; ++first) mbar_arrive(full + first % SLOTS);
       };
-      long long off = offset_of(u.i0);
+      // A tile whose tokens are all seen by some query comes as boxes, one page's tokens x 64 columns each, box pt by
+      // thread pt; others, and pages that do not divide a tile, row by row, with zeros for what nobody sees.
+      constexpr int COLS = D / 64;
+      const int n_boxes = w.page_rows ? T / w.page_rows * COLS : 0;
+      auto boxed = [&](int i) {
+        const int t = tile_token(rg, i, T);
+        return w.page_rows && t + T - 1 <= p_hi && (a.window == 0 || p_lo - t < a.window || t + T <= a.sinks);
+      };
+      auto box_page = [&](int i) {                    // page of this thread's box
+        return i < u.i1 && pt < n_boxes ? trow[page_of(a, tile_token(rg, i, T) + pt / COLS * w.page_rows)] : 0;
+      };
+      bool as_box = boxed(u.i0);
+      long long off = as_box ? -1 : offset_of(u.i0);
+      int page = as_box ? box_page(u.i0) : 0;
       for (int i = u.i0; i < u.i1 && ok; ++i) {
-        const long long off_next = offset_of(i + 1);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (kv >= SLOTS && !ready(empty + kv % SLOTS, kv / SLOTS - 1)) {
-            cp_async_wait_all();                       // nothing to issue: hand over what is on its way first
+        const bool box_next = i + 1 < u.i1 && boxed(i + 1);
+        const long long off_next = box_next ? -1 : offset_of(i + 1);
+        const int page_next = box_next ? box_page(i + 1) : 0;
+        if (as_box) {
+          if (first < kv || !q_given) {               // copies on their way go first
+            cp_async_wait_all();
             hand_over(kv);
-            ok = wait(empty + kv % SLOTS, kv / SLOTS - 1);
+            if (!q_given) {
+              q_given = true;
+              mbar_arrive(q_full);
+            }
           }
-          if (!ok) break;
-          const uint32_t dst = smem_u32(ring + (kv % SLOTS) * C::SLOT);
-          const uint16_t* base = x ? vh : kh;
-          constexpr int RPP = 32 / CPR > 0 ? 32 / CPR : 1, PASSES = (T / 4) * CPR / 32;
+          const int t0 = tile_token(rg, i, T) + pt / COLS * w.page_rows, in_page = t0 - page_of(a, t0) * a.page_size;
+          const uint32_t at = (pt % COLS) * (T * 128) + pt / COLS * w.page_rows * 128;
 #pragma unroll
-          for (int v = 0; v < PASSES; ++v) {
-            const int r = v * RPP + lane / CPR, c = lane % CPR;
-            const long long o = __shfl_sync(0xFFFFFFFFu, off, r);
-            const uint32_t row = pw * (T / 4) + r;
-            cp_async16(dst + (c >> 3) * (T * 128) + swz128(row, c & 7), base + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+          for (int x = 0; x < 2; ++x) {
+            if (ok && kv >= SLOTS && !wait(empty + kv % SLOTS, kv / SLOTS - 1)) ok = false;
+            if (!ok) break;
+            uint64_t* bar_full = full + kv % SLOTS;
+            if (pt >= n_boxes) {
+              mbar_arrive(bar_full);
+            } else if (page >= 0 && page < a.pages) {
+              mbar_expect_tx(bar_full, w.page_rows * 128);
+              tma_load_4d(smem_u32(ring + (kv % SLOTS) * C::SLOT) + at, x ? &maps.v : &maps.k, (pt % COLS) * 64, in_page, u.h, page,
+                          bar_full);
+            } else {                                  // a missing page reads as zeros
+              set_err(a.err, SSB_ERR_PAGE_RANGE);
+              uint4* z = (uint4*)(ring + (kv % SLOTS) * C::SLOT + at);
+              for (int y = 0; y < w.page_rows * 8; ++y) z[y] = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+              mbar_arrive(bar_full);
+            }
+            ++kv;
           }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          ++kv;
-          if (kv - first > LAG) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-            hand_over(kv - LAG);
+          first = kv;
+        } else {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ok && kv >= SLOTS && !ready(empty + kv % SLOTS, kv / SLOTS - 1)) {
+              cp_async_wait_all();                     // nothing to issue: hand over what is on its way first
+              hand_over(kv);
+              ok = wait(empty + kv % SLOTS, kv / SLOTS - 1);
+            }
+            if (!ok) break;
+            const uint32_t dst = smem_u32(ring + (kv % SLOTS) * C::SLOT);
+            const uint16_t* base = x ? vh : kh;
+            constexpr int RPP = 32 / CPR > 0 ? 32 / CPR : 1, PASSES = (T / 4) * CPR / 32;
+#pragma unroll 4
+            for (int v = 0; v < PASSES; ++v) {
+              const int r = v * RPP + lane / CPR, c = lane % CPR;
+              const long long o = __shfl_sync(0xFFFFFFFFu, off, r);
+              const uint32_t row = pw * (T / 4) + r;
+              cp_async16(dst + (c >> 3) * (T * 128) + swz128(row, c & 7), base + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++kv;
+            if (kv - first > LAG) {
+              asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
+              hand_over(kv - LAG);
+            }
           }
         }
         off = off_next;
+        page = page_next;
+        as_box = box_next;
       }
       cp_async_wait_all();
       if (ok) hand_over(kv);
     }
     cp_async_wait_all();
     if (!ok) give_up();
-  } else if (warp < PROD) {
+  } else {
+    if constexpr (C::P_IN_S) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFT));
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     Unit u;
     uint32_t tn = 0;
     bool ok = true;
+    if (NT == 2 && t == 1) mbar_arrive(turn);       // the first turn is row tile 0's
     while (ok && next_unit(u)) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
@@ -560,10 +661,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
           break;
         }
         tc_fence_after();
-        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * (T / 2);
+        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * C::P_STEP;
         const int tok = tile_token(rg, i, T);
         float v[T];
         tmem_ld_row<T>(sc, v);
+        if constexpr (!C::P_IN_S) {
+          tc_fence_before();
+          mbar_arrive(s_free + buf);
+        }
         if (!seen_by_all(a, tok, tok + T, t_lo, t_hi)) {
 #pragma unroll
           for (int c = 0; c < T; c += 16) {
@@ -585,10 +690,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
         if (i == u.i0) {
           m = mx;
         } else {
-          // The product of the tile before reads the P that is written next (with one row tile: the other buffer) and adds to
-          // the sum that may be rescaled. A parity wait sees one phase back only, so it is waited for at every tile.
+          // The product of the tile before adds to the sum that may be rescaled and reads the P that is written next (with
+          // one row tile: the other buffer). A parity wait sees one phase back only, so no tile goes by without one.
           const bool raise = mx > m + 8.f, any = __any_sync(0xFFFFFFFFu, raise);
-          if (NT == 2 || any) {
+          if ((NT == 2 && !C::P_IN_S) || any) {
             if (!warp_wait(o_done + t, tn - 1)) {
               ok = false;
               break;
@@ -611,6 +716,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
             }
           }
         }
+        // The two groups take turns at the exponentials, which the special-function units do at 16 a clock: in step, both
+        // would take twice as long and then both wait for the tensor cores.
+        if (NT == 2 && !warp_wait(turn + t, tn)) {
+          ok = false;
+          break;
+        }
         const float mu = m == -INFINITY ? 0.f : m;
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), mu2 = make_float2(-mu, -mu);
         float2 l2 = make_float2(0.f, 0.f), l3 = l2;
@@ -627,12 +738,20 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(Args a, Work w) 
             r[x] = pack2<E>(e.x, e.y);
           }
           tmem_st8(pc + c / 2, r);
+          if (C::P_IN_S && c + 16 == T / 2) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_half + buf);
+          }
         }
+        if (NT == 2) mbar_arrive(turn + (t ^ 1));
         l += (l2.x + l2.y) + (l3.x + l3.y);
         tmem_st_wait();
-        if (NT == 1 && pending && !warp_wait(o_done + t, tn - 1)) {
-          ok = false;
-          break;
+        if (NT == 1 && pending) {
+          if (!warp_wait(o_done + t, tn - 1)) {
+            ok = false;
+            break;
+          }
         }
         tc_fence_before();
         mbar_arrive(p_full + buf);
@@ -739,6 +858,52 @@ Layout layout_of(int dim, int n, int64_t rows, int heads, int kv_heads) {
   return l;
 }
 
+// The driver's tensor-map encoder, looked up through the runtime.
+using EncodeFn = decltype(&cuTensorMapEncodeTiled);
+EncodeFn encode_fn() {
+  static EncodeFn fn = []() -> EncodeFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+bool encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i + 1 < rank; ++i)                 // what the encoder refuses goes by cp.async
+    if (strides[i] == 0 || strides[i] >= (1ull << 40)) return false;
+  EncodeFn f = encode_fn();
+  return f && f(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims,
+                strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Boxes need pages that divide a tile or are divided by it, at least 8 tokens long (shorter ones would be many small
+// boxes), and a group that divides the 128 rows of a row tile.
+void make_maps(Maps& m, Work& w, const Args& a, bool bf16, int dim, int tile) {
+  w.page_rows = w.q_boxes = 0;
+  if (a.page_size >= 8 && (a.page_size & (a.page_size - 1)) == 0) {
+    const int rows = a.page_size < tile ? a.page_size : tile;
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)a.page_size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)a.st * 2, (cuuint64_t)a.sh * 2, (cuuint64_t)a.sp * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+    if (a.st > 0 && a.sh > 0 && a.sp > 0 && encode(&m.k, bf16, 4, a.k, dims, strides, box) &&
+        encode(&m.v, bf16, 4, a.v, dims, strides, box))
+      w.page_rows = rows;
+  }
+  if (128 % a.group == 0) {
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.heads, (cuuint64_t)a.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_tok * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(128 / a.group)};
+    w.q_boxes = a.q_head > 0 && a.q_tok > 0 && encode(&m.q, bf16, 3, a.q, dims, strides, box);
+  }
+}
+
 template <typename E, int D>
 int launch(Args& a, uint8_t* ws, const Layout& l, cudaStream_t stream) {
   using C = Cfg<D>;
@@ -757,11 +922,22 @@ int launch(Args& a, uint8_t* ws, const Layout& l, cudaStream_t stream) {
     (void)cudaGetLastError();
     return (int)e;
   }
+  if (C::P_IN_S) {                                   // the register split would wait forever for what the launch lacks
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, kern);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return (int)e;
+    }
+    if (at.numRegs != C::R_LAUNCH) return SSB_EUNSUPPORTED;
+  }
   ssb_note_smem("attn_prefill", kern, C::SMEM);
+  Maps maps = {};
+  make_maps(maps, w, a, sizeof(E) == 2 && idesc_of<E>(128, 64, false) == idesc_of<__nv_bfloat16>(128, 64, false), D, C::T);
   const int blocks = sm_count();
   int rc = ssb_launch(k_prefill_plan<C::MB, C::T>, dim3(1), dim3(PLAN_T), 0, stream, false, a, w, blocks);
   if (rc) return rc;
-  rc = ssb_launch(kern, dim3(blocks), dim3(C::THREADS), C::SMEM, stream, true, a, w);
+  rc = ssb_launch(kern, dim3(blocks), dim3(C::THREADS), C::SMEM, stream, true, maps, a, w);
   if (rc) return rc;
   return ssb_launch(k_prefill_join<E, D>, dim3(l.max_slots / 2, C::MB / 8), dim3(2 * D), 0, stream, true, a, w);
 }
