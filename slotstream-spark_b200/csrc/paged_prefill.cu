@@ -5,21 +5,23 @@
 // S = Q K^T from shared memory, and O += P V with P read from TMEM, where the softmax has put it.
 // What bounds it: the two products are 4 T MB D operations and the softmax T MB exponentials per tile; at head size
 // 128 the tensor cores and the 16 exponentials per clock of an SM need the same time, so both have to run all the time.
-// Hence two row tiles of 128 in turn (NT = 2): while one is in the softmax the other is in the products. At head size 256
-// one accumulator fills half of TMEM, so one row tile (NT = 1) alternates between two buffers of S instead: S of
-// the next tile is computed while the softmax works on this one.
+// Hence two row tiles of 128 (NT = 2; one at head size 256, whose accumulator fills half of TMEM) and two buffers of S for
+// each: the S of the next tile is computed under the softmax of this one, so neither waits for the latency of the other
+// (about 350 cycles from an instruction's issue to a waiting thread).
 //
 // The running maximum is only raised when a row's maximum grows by more than 2^8 (log2 domain): p stays below 2^8, which
 // both types and the fp32 sums hold with the same relative precision, and rescaling the accumulator in TMEM becomes rare.
 //
-// Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V rows through
-// cp.async (any page size; rows that no query sees become zeros) into 128-byte-swizzled tiles and hand out the units, and one
-// per row tile and product that issues its matrix instructions. Nothing orders products of different threads, shapes or
-// accumulators but the waits here. S is read into registers once. At sizes 64 and 256 tiles are 64 tokens, P has TMEM
-// columns of its own, and S is free as soon as it has been read: the next S runs under the exponentials. At 128 the
-// accumulators and two S of 128 tokens fill TMEM; P takes the place of S, the next S waits for the product that reads P, and
-// that product starts with the first half of P. (Shorter tiles cost the tensor cores more there: an instruction of 64 or 80
-// columns takes 48 or 54 cycles, bound by reading its operands from shared memory, one of 128 takes 64.)
+// Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V into
+// 128-byte-swizzled tiles (TMA boxes where pages allow, else row by row with cp.async; rows that no query sees become zeros) and
+// hand out the units, and one per row tile and product that issues its matrix instructions. Nothing orders products of
+// different threads, shapes or accumulators but the waits here. S is read into registers once and P takes its place; a
+// buffer is free for the next S when the product that read P has ended.
+//
+// Tiles of 64 tokens: two buffers of S for two row tiles of head size 128 fill TMEM. Instructions of 64 columns cost 48
+// cycles for 32 columns' worth of work (operands read from shared memory), so the products of a pair of tiles take 2570
+// cycles per 128 tokens instead of 2050; single-buffered tiles of 128, where each S waits for the product before it, took
+// 4600 (32K tokens, window 4096: 2.16 ms against 1.96).
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
@@ -35,17 +37,11 @@ namespace {
 
 template <int D>
 struct Cfg {
-  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = D == 128 ? 128 : 64, SLOTS = D == 64 ? 16 : 5;
+  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = 64, SLOTS = D == 64 ? 16 : D == 128 ? 10 : 5;
   static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
-  // TMEM columns: the accumulators, two buffers of S, two of P (two elements a column; in the place of S at size 128)
-  static constexpr bool P_IN_S = D == 128;
-  static constexpr int S_COL = NT * D, P_COL = P_IN_S ? S_COL : S_COL + 2 * T, P_STEP = P_IN_S ? T : T / 2;
-  static_assert(S_COL + 2 * T <= 512 && P_COL + P_STEP + T / 2 <= 512, "TMEM");
-  // With 128 columns of S in a softmax thread's registers, the softmax warps take some from the others:
-  // 256 x R_SOFT + 256 x R_REST = 512 x R_LAUNCH.
-  static constexpr int R_SOFT = 192, R_REST = 64, R_LAUNCH = 128;
-  static_assert(!P_IN_S || 256 * R_SOFT + 256 * R_REST == THREADS * R_LAUNCH, "registers");
+  static constexpr int S_COL = NT * D;             // TMEM columns: the accumulators, then two buffers of S / P a row tile
+  static_assert(S_COL + NT * 2 * T <= 512, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 1;
 
@@ -347,8 +343,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
   uint8_t* sq = smem;
   uint8_t* ring = smem + C::QB;
   uint64_t* bar = (uint64_t*)(ring + SLOTS * C::SLOT);
-  uint64_t *q_full = bar, *q_empty = bar + 1, *s_full = bar + 2, *s_free = bar + 4, *p_full = bar + 6, *o_done = bar + 8,
-           *u_full = bar + 10, *u_empty = bar + 12, *drained = bar + 14, *p_half = bar + 18, *turn = bar + 20, *full = bar + 22, *empty = full + SLOTS;
+  uint64_t *q_full = bar, *q_empty = bar + 1, *u_full = bar + 2, *u_empty = bar + 4, *drained = bar + 6,
+           *s_full = bar + 10, *p_full = bar + 14, *o_done = bar + 18, *full = bar + 22, *empty = full + SLOTS;
   int* u_slot = (int*)(empty + SLOTS);             // unit numbers handed out, two in flight
   uint32_t* tmem_slot = (uint32_t*)(u_slot + 2);
   int* failed = (int*)(tmem_slot + 1);
@@ -364,16 +360,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     mbar_init(q_full, 128);
     mbar_init(q_empty, NT);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(s_free + i, 128);
-      mbar_init(p_full + i, 128);
-      mbar_init(p_half + i, 128);
-      mbar_init(turn + i, 128);
-      mbar_init(o_done + i, 1);
       mbar_init(u_full + i, 1);
       mbar_init(u_empty + i, NT * 128 + 128 + 2 * NT);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(drained + i, 1);
+    for (int i = 0; i < 4; ++i) {                    // s_full, p_full, o_done: [row tile][buffer]
+      mbar_init(drained + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_done + i, 1);
+    }
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(full + i, 128);
       mbar_init(empty + i, NT);
@@ -407,11 +402,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     return range_of(a, p + u.r0 / a.group, p + (u.r0 + u.rows - 1) / a.group, T);
   };
 
-  auto few_registers = [] {
-    if constexpr (C::P_IN_S) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
-  };
   if (warp >= MMA) {
-   few_registers();
    if (warp < MMA + 2 * NT && lane == 0) {
     // One warp per row tile and product: a thread that waits on a barrier between two products leaves the tensor cores
     // idle for about 170 cycles (its queue is short), unless another thread's products fill the gap.
@@ -420,6 +411,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     const bool scores = warp < MMA + NT;
     const uint32_t q_lo = desc_lo(smem_u32(sq) + t * 128 * 128, LEAD_K), k_lo = desc_lo(smem_u32(ring), LEAD_K),
                    v_lo = desc_lo(smem_u32(ring), T * 128);
+    // A commit costs the tensor cores about 40 cycles. With a long ring its slots are given back by plain arrivals, when a
+    // later wait shows that the product has ended; with a short one (size 256) that would be too late.
+    constexpr bool FREE_BY_COMMIT = SLOTS < 8;
     Unit u;
     uint32_t kv = 0, qn = 0, tn = 0;                // slots, units and tiles so far
     bool ok = true;
@@ -428,44 +422,33 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       if (scores) need(q_full, qn++);
 #pragma unroll 1
       for (int i = u.i0; i < u.i1 && ok; ++i, ++tn, kv += 2) {
-        const uint32_t buf = NT == 2 ? t : tn & 1, use = NT == 2 ? tn : tn >> 1;
+        const uint32_t buf = 2 * t + (tn & 1), use = tn >> 1, sd = tmem + C::S_COL + buf * T;
         if (scores) {
           const uint32_t slot = kv % SLOTS;
           need(full + slot, kv / SLOTS);
-          // what is in this buffer has been read: S by the softmax, or the P in its place by the product before
-          if (C::P_IN_S) {
-            if (tn) need(o_done + t, tn - 1);
-          } else if (use) {
-            need(s_free + buf, use - 1);
-          }
+          if (use) need(o_done + buf, use - 1);     // the product that read P from this buffer
           if (!ok) break;
+          if (!FREE_BY_COMMIT && tn >= 2) mbar_arrive(empty + (kv - 3) % SLOTS);      // and the values of two tiles before
           tc_fence_after();
-          const uint32_t kd = k_lo + slot * (C::SLOT >> 4), sd = tmem + C::S_COL + buf * T;
+          const uint32_t kd = k_lo + slot * (C::SLOT >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), kd + (((k / 4) * (T * 128) + (k % 4) * 32) >> 4),
                     ID_S, k > 0);
           umma_commit(s_full + buf);
-          umma_commit(empty + slot);
+          if (FREE_BY_COMMIT) umma_commit(empty + slot);
         } else {
           const uint32_t slot = (kv + 1) % SLOTS;
           need(full + slot, (kv + 1) / SLOTS);
-          const uint32_t vd = v_lo + slot * (C::SLOT >> 4), pd = tmem + C::P_COL + buf * C::P_STEP, od = tmem + t * D;
-          constexpr int HALF = C::P_IN_S ? T / 32 : 0;   // k steps that can start with the first half of P
-          if constexpr (HALF > 0) {
-            need(p_half + buf, use);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < HALF; ++k) umma_ts(od, pd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
-          }
           need(p_full + buf, use);
           if (!ok) break;
+          if (!FREE_BY_COMMIT) mbar_arrive(empty + kv % SLOTS);                       // S has been read: so have the keys
           tc_fence_after();
+          const uint32_t vd = v_lo + slot * (C::SLOT >> 4), od = tmem + t * D;
 #pragma unroll
-          for (int k = HALF; k < T / 16; ++k) umma_ts(od, pd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
-          umma_commit(o_done + t);
-          umma_commit(empty + slot);
+          for (int k = 0; k < T / 16; ++k) umma_ts(od, sd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
+          umma_commit(o_done + buf);
+          if (FREE_BY_COMMIT) umma_commit(empty + slot);
         }
       }
       if (scores && ok) umma_commit(q_empty);
@@ -475,7 +458,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     if (!wait(drained + (warp - MMA), 0)) give_up();
    }
   } else if (warp >= PROD) {
-    few_registers();
     const int pt = tid - PROD * 32, pw = pt >> 5;
     Unit u;
     uint32_t kv = 0, qn = 0;
@@ -641,13 +623,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     cp_async_wait_all();
     if (!ok) give_up();
   } else {
-    if constexpr (C::P_IN_S) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFT));
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     Unit u;
     uint32_t tn = 0;
     bool ok = true;
-    if (NT == 2 && t == 1) mbar_arrive(turn);       // the first turn is row tile 0's
     while (ok && next_unit(u)) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
@@ -655,20 +635,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
       float m = -INFINITY, l = 0.f;
       for (int i = u.i0; i < u.i1; ++i, ++tn) {
-        const int buf = NT == 2 ? t : tn & 1;
-        if (!warp_wait(s_full + buf, NT == 2 ? tn : tn >> 1)) {
+        const uint32_t buf = 2 * t + (tn & 1), sc = lane_base + C::S_COL + buf * T;
+        if (!warp_wait(s_full + buf, tn >> 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t sc = lane_base + C::S_COL + buf * T, pc = lane_base + C::P_COL + buf * C::P_STEP;
         const int tok = tile_token(rg, i, T);
         float v[T];
         tmem_ld_row<T>(sc, v);
-        if constexpr (!C::P_IN_S) {
-          tc_fence_before();
-          mbar_arrive(s_free + buf);
-        }
         if (!seen_by_all(a, tok, tok + T, t_lo, t_hi)) {
 #pragma unroll
           for (int c = 0; c < T; c += 16) {
@@ -686,21 +661,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
             m4[y] = x + 4 + y < T ? fmaxf(m4[y], fmaxf(v[x + y], v[x + 4 + y])) : fmaxf(m4[y], v[x + y]);
         }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
-        bool pending = i > u.i0;
         if (i == u.i0) {
           m = mx;
         } else {
-          // The product of the tile before adds to the sum that may be rescaled and reads the P that is written next (with
-          // one row tile: the other buffer). A parity wait sees one phase back only, so no tile goes by without one.
-          const bool raise = mx > m + 8.f, any = __any_sync(0xFFFFFFFFu, raise);
-          if ((NT == 2 && !C::P_IN_S) || any) {
-            if (!warp_wait(o_done + t, tn - 1)) {
+          const bool raise = mx > m + 8.f;
+          if (__any_sync(0xFFFFFFFFu, raise)) {
+            if (!warp_wait(o_done + (buf ^ 1), (tn - 1) >> 1)) {     // the product of the tile before adds to the sum
               ok = false;
               break;
             }
-            pending = false;
-          }
-          if (any) {
             tc_fence_after();
             const float f = raise ? ex2(m - mx) : 1.f;
             if (raise) m = mx;
@@ -715,12 +684,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
               tmem_st16(lane_base + t * D + c, r);
             }
           }
-        }
-        // The two groups take turns at the exponentials, which the special-function units do at 16 a clock: in step, both
-        // would take twice as long and then both wait for the tensor cores.
-        if (NT == 2 && !warp_wait(turn + t, tn)) {
-          ok = false;
-          break;
         }
         const float mu = m == -INFINITY ? 0.f : m;
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), mu2 = make_float2(-mu, -mu);
@@ -737,26 +700,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
             else l2 = __fadd2_rn(l2, e);
             r[x] = pack2<E>(e.x, e.y);
           }
-          tmem_st8(pc + c / 2, r);
-          if (C::P_IN_S && c + 16 == T / 2) {
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(p_half + buf);
-          }
+          tmem_st8(sc + c / 2, r);               // P takes the place of S, which is in registers
         }
-        if (NT == 2) mbar_arrive(turn + (t ^ 1));
         l += (l2.x + l2.y) + (l3.x + l3.y);
         tmem_st_wait();
-        if (NT == 1 && pending) {
-          if (!warp_wait(o_done + t, tn - 1)) {
-            ok = false;
-            break;
-          }
-        }
         tc_fence_before();
         mbar_arrive(p_full + buf);
       }
-      if (!ok || !warp_wait(o_done + t, tn - 1)) {
+      if (!ok || !warp_wait(o_done + 2 * t + ((tn - 1) & 1), (tn - 1) >> 1)) {
         ok = false;
         break;
       }
@@ -921,15 +872,6 @@ int launch(Args& a, uint8_t* ws, const Layout& l, cudaStream_t stream) {
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return (int)e;
-  }
-  if (C::P_IN_S) {                                   // the register split would wait forever for what the launch lacks
-    cudaFuncAttributes at;
-    e = cudaFuncGetAttributes(&at, kern);
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return (int)e;
-    }
-    if (at.numRegs != C::R_LAUNCH) return SSB_EUNSUPPORTED;
   }
   ssb_note_smem("attn_prefill", kern, C::SMEM);
   Maps maps = {};
