@@ -13,6 +13,7 @@
 namespace {
 
 constexpr int PLAN_T = 1024;
+constexpr int BITMAP = 65536 / 8;         // shared memory for one bit per sequence, at most
 constexpr int MAX_PAGES = 1 << 20;   // PLAN_T sequences that each lack them all still sum within an int32
 
 struct Cache {
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
 
 __global__ void __launch_bounds__(PLAN_T) k_fork_plan(Cache c, const int32_t* __restrict__ parents,
                                                       const int32_t* __restrict__ children, int n) {
+  pdl_trigger();
   extern __shared__ uint32_t bitmap[];
   __shared__ int part[33];
   __shared__ int bad;
@@ -312,6 +314,7 @@ __global__ void __launch_bounds__(256) k_free(Cache c, const int32_t* __restrict
 }
 
 __global__ void __launch_bounds__(PLAN_T) k_compact_plan(Cache c) {
+  pdl_trigger();
   __shared__ int part[33];
   const Scratch sc = scratch_of(c);
   const WordSpan ws = word_span(c.pages);
@@ -429,13 +432,6 @@ int cache_of(const ssb_kv_cache* c, Cache* o) {
   return SSB_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 }  // namespace
 
 extern "C" int ssb_kv_scratch_ints(int32_t pages, int32_t seqs) {
@@ -451,7 +447,8 @@ extern "C" int ssb_kv_extend(const ssb_kv_cache* cc, const int32_t* ids, const i
   if (n == 0) return SSB_OK;
   SSB_CHECK_ARG(ids && counts);
   const size_t smem = (size_t)((c.seqs + 31) / 32) * 4;
-  ssb_note_smem("kv_extend", k_extend, smem);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ssb_setup_kernel(done, "kv_extend", k_extend, BITMAP)) return rc;
   return ssb_launch(k_extend, dim3(1), dim3(PLAN_T), smem, (cudaStream_t)stream, false, c, ids, counts, n);
 }
 
@@ -463,10 +460,11 @@ extern "C" int ssb_kv_fork(const ssb_kv_cache* cc, const int32_t* parents, const
   if (n == 0) return SSB_OK;
   SSB_CHECK_ARG(parents && children);
   const size_t smem = (size_t)((c.seqs + 31) / 32) * 4;
-  ssb_note_smem("kv_fork", k_fork_plan, smem);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ssb_setup_kernel(done, "kv_fork", k_fork_plan, BITMAP)) return rc;
   int rc = ssb_launch(k_fork_plan, dim3(1), dim3(PLAN_T), smem, (cudaStream_t)stream, false, c, parents, children, n);
   if (rc) return rc;
-  const int64_t tasks = (int64_t)n * ((c.page_bytes + PIECE - 1) / PIECE), most = (int64_t)sm_count() * 8;
+  const int64_t tasks = (int64_t)n * ((c.page_bytes + PIECE - 1) / PIECE), most = (int64_t)ssb_sm_count() * 8;
   return ssb_launch(k_fork_apply, dim3((unsigned)(tasks < most ? tasks : most)), dim3(COPY_T), 0, (cudaStream_t)stream,
                     true, c, parents, children);
 }
@@ -479,7 +477,8 @@ extern "C" int ssb_kv_free(const ssb_kv_cache* cc, const int32_t* ids, const int
   if (n == 0) return SSB_OK;
   SSB_CHECK_ARG(ids);
   SSB_CHECK_ARG(c.max_pages <= 65535 * 1024);
-  ssb_note_smem("kv_free", k_free, 0);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ssb_setup_kernel(done, "kv_free", k_free, 0)) return rc;
   return ssb_launch(k_free, dim3((unsigned)n, (unsigned)((c.max_pages + 1023) / 1024)), dim3(256), 0,
                     (cudaStream_t)stream, false, c, ids, first, last);
 }
@@ -487,10 +486,11 @@ extern "C" int ssb_kv_free(const ssb_kv_cache* cc, const int32_t* ids, const int
 extern "C" int ssb_kv_compact(const ssb_kv_cache* cc, void* stream) {
   Cache c;
   if (int rc = cache_of(cc, &c)) return rc;
-  ssb_note_smem("kv_compact", k_compact_plan, 0);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ssb_setup_kernel(done, "kv_compact", k_compact_plan, 0)) return rc;
   int rc = ssb_launch(k_compact_plan, dim3(1), dim3(PLAN_T), 0, (cudaStream_t)stream, false, c);
   if (rc) return rc;
-  return ssb_launch(k_compact_apply, dim3((unsigned)sm_count() * 8), dim3(COPY_T), 0, (cudaStream_t)stream, true, c);
+  return ssb_launch(k_compact_apply, dim3((unsigned)ssb_sm_count() * 8), dim3(COPY_T), 0, (cudaStream_t)stream, true, c);
 }
 
 extern "C" int ssb_kv_write(const ssb_kv_cache* cc, const uint16_t* k, const uint16_t* v, int64_t rows,
@@ -510,6 +510,7 @@ extern "C" int ssb_kv_write(const ssb_kv_cache* cc, const uint16_t* k, const uin
   SSB_CHECK_ARG((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_layer | (uintptr_t)v_layer) & 15) == 0);
   WriteArgs a{k, v, rows, k_row_stride, k_head_stride, v_row_stride, v_head_stride, kv_heads, dim, starts, ids, n,
               k_layer, v_layer, page_stride, head_stride, token_stride};
-  ssb_note_smem("kv_write", k_write, 0);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ssb_setup_kernel(done, "kv_write", k_write, 0)) return rc;
   return ssb_launch(k_write, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, false, c, a);
 }

@@ -4,10 +4,13 @@
 // log2 domain), o = p v. The rows of one key head -- query tokens x heads of its group -- share every key and value
 // read, so each cached byte is read once per key head: the kernel is bound by reading the cache. Tensor cores
 // (mma.sync m16n8k16, fp32 accumulation) do both products, since RB x D x 2 multiply-adds per cached element pair
-// would otherwise take more issue slots than the loads leave; tcgen05's 128-row tiles would be mostly padding here.
+// would otherwise take more issue slots than the loads leave; tcgen05's 128-row tiles would be mostly padding here. The
+// products are taken transposed -- S^T = K Q^T, O^T = V^T P^T -- so that the query rows are the instruction's 8 columns
+// and nothing is padded to 16 for groups of up to eight rows (at 131,072 tokens and head size 256, 84 us with rows padded to
+// 16, REPLACE us now).
 //
-// A block has NW warps that work alone: each walks every NW-th sub-tile of TW tokens through its own ring of NS
-// cp.async stages (no block barrier inside an item), and the warps' (max, sum, accumulator) are joined through shared
+// A block has NW warps that work alone: each walks every NW-th sub-tile of TW tokens through its own ring of cp.async
+// units (no block barrier inside an item), and the warps' (max, sum, accumulator) are joined through shared
 // memory at the end of the item. p is rounded to the inputs' type for the second product (relative 2^-8 for bf16,
 // 2^-11 for fp16, as the library's other tensor-core inputs); its sum is taken before the rounding, in fp32.
 #include "paged_attn.cuh"
@@ -27,6 +30,12 @@ SSB_DEV void ldsm4t(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held two a thread.
+SSB_DEV uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <typename E>
 SSB_DEV void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -54,84 +63,87 @@ SSB_DEV uint32_t swz(int r, int c) {
   return (uint32_t)(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
-constexpr int NW = 4, RB = 16, NS = 3;
+constexpr int NW = 4;
 template <int D>
-constexpr int TW = D == 64 ? 32 : 16;
+constexpr int TW = D == 256 ? 16 : 32;            // tokens of a warp's sub-tile
 template <int D>
-constexpr int STAGE = TW<D> * D * 2 * 2;          // keys and values of one sub-tile
+constexpr int UNIT = TW<D> * D * 2;               // keys, or values, of one sub-tile
 template <int D>
-constexpr int SMEM = RB * D * 2 + NW * NS * STAGE<D>;
-template <int D>
-constexpr int BLOCKS_PER_SM = D == 256 ? 1 : 2;
+constexpr int NU = D == 64 ? 6 : 3;               // units in a warp's ring: 24 KB, all but one in flight
+template <int D, int RB>
+constexpr int SMEM = RB * D * 2 + NW * NU<D> * UNIT<D>;
+constexpr int BLOCKS_PER_SM = 2;
 
-template <typename E, int D>
-__global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM<D>) k_attn_rows(Args a) {
-  constexpr int T = NW * TW<D>, CPR = D / 8;       // tokens of a tile, 16-byte chunks of a row
+template <typename E, int D, int RB>
+__global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
+  constexpr int T = NW * TW<D>, CPR = D / 8, NB = RB / 8;       // tokens of a tile, 16-byte chunks and blocks of 8 rows
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long scan[NW + 1];
-  __shared__ long long plan[3];                    // chunk, then the item where this block starts: its start, b
+  __shared__ long long scan[NW];
+  __shared__ long long place[2];                   // the sequence where this block starts, and its first tile
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t* sq = smem;
-  uint8_t* ring = smem + RB * D * 2 + warp * NS * STAGE<D>;
+  uint8_t* ring = smem + RB * D * 2 + warp * NU<D> * UNIT<D>;
   pdl_wait();
+  pdl_trigger();                                   // the join's blocks may come up; they wait for this grid's end
 
-  // ---- this block's share: tiles of all sequences, divided evenly
-  auto tiles_of = [&](int b, int* items, int* tiles) {
+  // ---- this block's share: tiles of all sequences, divided evenly. One scan of the sequences' weights for each NW * 32 of
+  // them; where they all fit in one, it gives the total and the place of this block's first tile at once.
+  auto weight_of = [&](int b) -> long long {
+    if (b >= a.n) return 0;
     const Seq s = seq_of(a, b);
-    *items = a.kv_heads * ((s.q * a.group + RB - 1) / RB);
-    *tiles = range_of(a, s.len - s.q, s.len - 1, T).tiles;
+    return (long long)a.kv_heads * ((s.q * a.group + RB - 1) / RB) * range_of(a, s.len - s.q, s.len - 1, T).tiles;
   };
-  long long mine = 0;
-  for (int b = tid; b < a.n; b += NW * 32) {
-    int items, tiles;
-    tiles_of(b, &items, &tiles);
-    mine += (long long)items * tiles;
-  }
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-  if (lane == 0) scan[warp] = mine;
-  __syncthreads();
-  if (tid == 0) {
-    long long t = 0;
-    for (int w = 0; w < NW; ++w) t += scan[w];
-    const long long ch = (t + gridDim.x - 1) / gridDim.x;
-    plan[0] = ch < 2 ? 2 : ch;
-    plan[1] = t;
-    a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  }
-  __syncthreads();
-  const long long chunk = plan[0], total = plan[1];
-  const long long lo = chunk * blockIdx.x, hi = min(lo + chunk, total);
-  if (lo >= hi) return;
-  // the sequence that holds tile `lo`
-  int b = 0;
-  long long begin = 0;
-  for (int b0 = 0;; b0 += NW * 32) {
-    int items = 0, tiles = 0;
-    if (b0 + tid < a.n) tiles_of(b0 + tid, &items, &tiles);
-    long long w = (long long)items * tiles, inc = w;
+  auto scan_block = [&](long long w, long long* sum) {      // inclusive
+    long long inc = w;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      long long u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      const long long u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
       if (lane >= o) inc += u;
     }
     __syncthreads();
     if (lane == 31) scan[warp] = inc;
-    if (tid == 0) scan[NW] = -1;
     __syncthreads();
-    long long pre = begin;
-    for (int v = 0; v < warp; ++v) pre += scan[v];
-    if (lo >= pre + inc - w && lo < pre + inc) {
-      plan[1] = pre + inc - w;
-      scan[NW] = b0 + tid;
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      if (v < warp) before += scan[v];
+      all += scan[v];
     }
-    __syncthreads();
-    if (scan[NW] >= 0) {
-      b = (int)scan[NW];
-      begin = plan[1];
-      break;
-    }
-    for (int v = 0; v < NW; ++v) begin += scan[v];
-    __syncthreads();
+    *sum = all;
+    return before + inc;
+  };
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  long long w0 = weight_of(tid), total;
+  const long long inc0 = scan_block(w0, &total);
+  const long long first_total = total;
+  if (a.n > NW * 32) {
+    long long more = 0;
+    for (int b = tid + NW * 32; b < a.n; b += NW * 32) more += weight_of(b);
+    long long rest;
+    scan_block(more, &rest);
+    total += rest;
   }
+  const long long chunk = max((total + gridDim.x - 1) / gridDim.x, 1ll);
+  const long long lo = chunk * blockIdx.x, hi = min(lo + chunk, total);
+  if (lo >= hi) return;
+  // the sequence that holds tile `lo`, and its first tile
+  if (lo >= inc0 - w0 && lo < inc0) {
+    place[0] = tid;
+    place[1] = inc0 - w0;
+  }
+  long long seen_total = first_total;
+  for (int b0 = NW * 32; lo >= seen_total; b0 += NW * 32) {
+    long long sum;
+    const long long w = weight_of(b0 + tid), inc = seen_total + scan_block(w, &sum);
+    if (lo >= inc - w && lo < inc) {
+      place[0] = b0 + tid;
+      place[1] = inc - w;
+    }
+    seen_total += sum;
+  }
+  __syncthreads();
+  int b = (int)place[0];
+  long long begin = place[1];
 
   long long at = lo;
   Seq s = seq_of(a, b);
@@ -175,126 +187,211 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM<D>) k_attn_rows(Args a)
       }
       return (long long)page * a.sp + (long long)(t - j * a.page_size) * a.st;
     };
-    auto issue = [&](int i, int slot) {
-      uint8_t* st = ring + slot * STAGE<D>;
-      const int t0 = tile_token(rg, i, T) + warp * TW<D>;
-      long long mine_off = lane < TW<D> ? offset_of(t0 + lane) : -1;
+    // Unit n of this part: keys (n even) or values (n odd) of tile i0 + n / 2. Lane l holds the offset of token l; values
+    // are issued right after their keys and use the same.
+    const int n_units = 2 * (i1 - i0);
+    long long mine_off = -1;
+    auto issue = [&](int n) {
+      if (n < n_units) {
+        if ((n & 1) == 0) mine_off = lane < TW<D> ? offset_of(tile_token(rg, i0 + (n >> 1), T) + warp * TW<D> + lane) : -1;
+        const uint32_t dst = smem_u32(ring + n % NU<D> * UNIT<D>);
+        const uint16_t* base = n & 1 ? vh : kh;
 #pragma unroll
-      for (int u = 0; u < TW<D> * CPR / 32; ++u) {
-        const int r = (u * 32 + lane) / CPR, c = (u * 32 + lane) % CPR;
-        const long long off = __shfl_sync(0xFFFFFFFFu, mine_off, r);
-        const uint32_t n = off < 0 ? 0 : 16;
-        const uint16_t* src = kh + (off < 0 ? 0 : off) + c * 8;
-        const uint16_t* srv = vh + (off < 0 ? 0 : off) + c * 8;
-        cp_async16(smem_u32(st) + swz<D>(r, c), src, n);
-        cp_async16(smem_u32(st) + STAGE<D> / 2 + swz<D>(r, c), srv, n);
+        for (int u = 0; u < TW<D> * CPR / 32; ++u) {
+          const int r = (u * 32 + lane) / CPR, c = (u * 32 + lane) % CPR;
+          const long long off = __shfl_sync(0xFFFFFFFFu, mine_off, r);
+          cp_async16(dst + swz<D>(r, c), base + (off < 0 ? 0 : off) + c * 8, off < 0 ? 0 : 16);
+        }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto landed = [&] {                              // the oldest unit in flight is there, for every lane
+      asm volatile("cp.async.wait_group %0;" ::"n"(NU<D> - 2) : "memory");
+      __syncwarp();
     };
 
-    float acc[D / 8][4];
+    // Rows are the columns of both products (see the top): a thread holds rows 8 n + 2 (lane % 4) and the next of every
+    // n < NB, as columns of S^T (tokens lane / 4 and + 8 of a group of 16) and of O^T (dims lane / 4 and + 8 of 16).
+    constexpr int MT = TW<D> / 16, KS = D / 16;
+    constexpr bool Q_IN_REGS = KS * NB <= 16;
+    float acc[KS][NB][4];
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    const int ra = lane >> 2, rb8 = ra + 8;
-    // rows past the item's last have zero queries and are never written: they take the last one's position
-    const int pa = p_first + (r0 + min(ra, rows - 1)) / a.group, pb = p_first + (r0 + min(rb8, rows - 1)) / a.group;
+    for (int j = 0; j < KS; ++j)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
+    float m[NB][2], l[NB][2];
+    int pos[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        m[n][y] = -INFINITY;
+        l[n][y] = 0.f;
+        // rows past the item's last have zero queries and are never written: they take the last one's position
+        pos[n][y] = p_first + (r0 + min(n * 8 + (lane & 3) * 2 + y, rows - 1)) / a.group;
+      }
+    auto load_q = [&](int kk, int n, uint32_t* b) {  // two steps of 16 dims: b[0..1] of kk, b[2..3] of kk + 1
+      ldsm4(smem_u32(sq) + swz<D>(n * 8 + (lane & 7), 2 * kk + (lane >> 3)), b);
+    };
+    uint32_t qf[Q_IN_REGS ? KS : 2][NB][2];
+    if constexpr (Q_IN_REGS) {
+#pragma unroll
+      for (int kk = 0; kk < KS; kk += 2)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          uint32_t b[4];
+          load_q(kk, n, b);
+          qf[kk][n][0] = b[0];
+          qf[kk][n][1] = b[1];
+          qf[kk + 1][n][0] = b[2];
+          qf[kk + 1][n][1] = b[3];
+        }
+    }
 
 #pragma unroll
-    for (int u = 0; u < NS - 1; ++u) {
-      if (i0 + u < i1) issue(i0 + u, u);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    for (int n = 0; n < NU<D> - 1; ++n) issue(n);
     for (int i = i0; i < i1; ++i) {
-      const int slot = (i - i0) % NS;
-      asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
-      __syncwarp();
-      const uint32_t ks = smem_u32(ring + slot * STAGE<D>), vs = ks + STAGE<D> / 2;
+      const int un = 2 * (i - i0);
+      landed();
+      const uint32_t ks = smem_u32(ring + un % NU<D> * UNIT<D>);
       const int t0 = tile_token(rg, i, T) + warp * TW<D>;
+      float c[MT][NB][4], c2[MT][NB][4];              // even and odd steps: two chains hide the instruction's latency
 #pragma unroll
-      for (int hf = 0; hf < TW<D> / 16; ++hf) {
-        float c[2][4] = {};
+      for (int x = 0; x < MT; ++x)
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t qa[4], kb[4];
-          ldsm4(smem_u32(sq) + swz<D>(lane & 15, 2 * kk + (lane >> 4)), qa);
-          ldsm4(ks + swz<D>(hf * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), kb);
-          mma16816<E>(c[0], qa, kb[0], kb[1]);
-          mma16816<E>(c[1], qa, kb[2], kb[3]);
-        }
-        const int t1 = t0 + hf * 16;
-        const bool whole = seen_by_all(a, t1, t1 + 16, p_lo, p_hi);
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+          for (int y = 0; y < 4; ++y) c[x][n][y] = c2[x][n][y] = 0.f;
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int t = t1 + x * 8 + (lane & 3) * 2 + y;
-            c[x][y] = whole || seen(a, t, pa) ? c[x][y] * a.scale_log2 : -INFINITY;
-            c[x][2 + y] = whole || seen(a, t, pb) ? c[x][2 + y] * a.scale_log2 : -INFINITY;
+      for (int kk = 0; kk < KS; kk += 2) {
+        if constexpr (!Q_IN_REGS) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            uint32_t b[4];
+            load_q(kk, n, b);
+            qf[0][n][0] = b[0];
+            qf[0][n][1] = b[1];
+            qf[1][n][0] = b[2];
+            qf[1][n][1] = b[3];
           }
-        float ma = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
-        float mb = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
-        ma = fmaxf(ma, __shfl_xor_sync(0xFFFFFFFFu, ma, 1));
-        mb = fmaxf(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, 1));
-        ma = fmaxf(m0, fmaxf(ma, __shfl_xor_sync(0xFFFFFFFFu, ma, 2)));
-        mb = fmaxf(m1, fmaxf(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, 2)));
-        if (__any_sync(0xFFFFFFFFu, ma != m0 || mb != m1)) {
-          const float fa = ma == m0 ? 1.f : ex2(m0 - ma), fb = mb == m1 ? 1.f : ex2(m1 - mb);
-          l0 *= fa;
-          l1 *= fb;
+        }
+        constexpr int Q0 = Q_IN_REGS ? 1 : 0;
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            acc[j][0] *= fa;
-            acc[j][1] *= fa;
-            acc[j][2] *= fb;
-            acc[j][3] *= fb;
+        for (int x = 0; x < MT; ++x) {
+          uint32_t ka[4], kb[4];
+          ldsm4(ks + swz<D>(x * 16 + (lane & 15), 2 * kk + (lane >> 4)), ka);
+          ldsm4(ks + swz<D>(x * 16 + (lane & 15), 2 * kk + 2 + (lane >> 4)), kb);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            mma16816<E>(c[x][n], ka, qf[Q0 * kk][n][0], qf[Q0 * kk][n][1]);
+            mma16816<E>(c2[x][n], kb, qf[Q0 * kk + 1][n][0], qf[Q0 * kk + 1][n][1]);
           }
-          m0 = ma;
-          m1 = mb;
-        }
-        const float ua = m0 == -INFINITY ? 0.f : m0, ub = m1 == -INFINITY ? 0.f : m1;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          c[x][0] = ex2(c[x][0] - ua);
-          c[x][1] = ex2(c[x][1] - ua);
-          c[x][2] = ex2(c[x][2] - ub);
-          c[x][3] = ex2(c[x][3] - ub);
-          l0 += c[x][0] + c[x][1];
-          l1 += c[x][2] + c[x][3];
-        }
-        const uint32_t p[4] = {pack2<E>(c[0][0], c[0][1]), pack2<E>(c[0][2], c[0][3]), pack2<E>(c[1][0], c[1][1]),
-                               pack2<E>(c[1][2], c[1][3])};
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          uint32_t vb[4];
-          ldsm4t(vs + swz<D>(hf * 16 + (lane & 15), 2 * j + (lane >> 4)), vb);
-          mma16816<E>(acc[2 * j], p, vb[0], vb[1]);
-          mma16816<E>(acc[2 * j + 1], p, vb[2], vb[3]);
         }
       }
       __syncwarp();
-      if (i + NS - 1 < i1) issue(i + NS - 1, (i - i0 + NS - 1) % NS);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      issue(un + NU<D> - 1);
+      // mask and scale; then the tile's maximum, one rescaling of what is there, and the weights
+      float top[NB][2];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+        const bool whole = seen_by_all(a, t0 + x * 16, t0 + x * 16 + 16, p_lo, p_hi);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int t = t0 + x * 16 + (lane >> 2) + (y >> 1) * 8;
+            const float v = c[x][n][y] + c2[x][n][y];
+            c[x][n][y] = whole || seen(a, t, pos[n][y & 1]) ? v * a.scale_log2 : -INFINITY;
+            top[n][y & 1] = fmaxf(top[n][y & 1], c[x][n][y]);
+          }
+      }
+      bool up = false;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float v = top[n][y];
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+          top[n][y] = fmaxf(v, m[n][y]);
+          up |= top[n][y] != m[n][y];
+        }
+      if (__any_sync(0xFFFFFFFFu, up)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float f = top[n][y] == m[n][y] ? 1.f : ex2(m[n][y] - top[n][y]);
+            m[n][y] = top[n][y];
+            l[n][y] *= f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              acc[j][n][y] *= f;
+              acc[j][n][2 + y] *= f;
+            }
+          }
+      }
+      uint32_t p[MT][NB][2];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const float u0 = m[n][0] == -INFINITY ? 0.f : m[n][0], u1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+        for (int x = 0; x < MT; ++x) {
+          float* e = c[x][n];
+          e[0] = ex2(e[0] - u0);
+          e[1] = ex2(e[1] - u1);
+          e[2] = ex2(e[2] - u0);
+          e[3] = ex2(e[3] - u1);
+          l[n][0] += e[0] + e[2];
+          l[n][1] += e[1] + e[3];
+          p[x][n][0] = transpose8(pack2<E>(e[0], e[1]));   // [8 tokens][8 rows] -> the second product's columns
+          p[x][n][1] = transpose8(pack2<E>(e[2], e[3]));
+        }
+      }
+      landed();
+      const uint32_t vs = smem_u32(ring + (un + 1) % NU<D> * UNIT<D>);
+#pragma unroll
+      for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          uint32_t va[4];
+          ldsm4t(vs + swz<D>(x * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)), va);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) mma16816<E>(acc[j][n], va, p[x][n][0], p[x][n][1]);
+        }
+      __syncwarp();
+      issue(un + NU<D>);
     }
-    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
-    l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
-    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
-    l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        l[n][y] += __shfl_xor_sync(0xFFFFFFFFu, l[n][y], 4);
+        l[n][y] += __shfl_xor_sync(0xFFFFFFFFu, l[n][y], 8);
+        l[n][y] += __shfl_xor_sync(0xFFFFFFFFu, l[n][y], 16);
+      }
 
     // ---- join the warps: their accumulators go through the (now idle) ring
     cp_async_wait_all();
     __syncthreads();
     float* wacc = (float*)(smem + RB * D * 2);                         // [NW][RB][D]
     float2* wml = (float2*)(wacc + NW * RB * D);                        // [NW][RB]
-    static_assert(NW * RB * D * 4 + NW * RB * 8 <= NW * NS * STAGE<D>, "the join needs the ring");
+    static_assert(NW * RB * D * 4 + NW * RB * 8 <= NW * NU<D> * UNIT<D>, "the join needs the ring");
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      *(float2*)(wacc + (warp * RB + ra) * D + j * 8 + (lane & 3) * 2) = make_float2(acc[j][0], acc[j][1]);
-      *(float2*)(wacc + (warp * RB + rb8) * D + j * 8 + (lane & 3) * 2) = make_float2(acc[j][2], acc[j][3]);
-    }
-    if ((lane & 3) == 0) {
-      wml[warp * RB + ra] = make_float2(m0, l0);
-      wml[warp * RB + rb8] = make_float2(m1, l1);
-    }
+    for (int j = 0; j < KS; ++j)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          wacc[(warp * RB + n * 8 + (lane & 3) * 2 + (y & 1)) * D + j * 16 + (lane >> 2) + (y >> 1) * 8] = acc[j][n][y];
+    if (lane < 4)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) wml[warp * RB + n * 8 + lane * 2 + y] = make_float2(m[n][y], l[n][y]);
     __syncthreads();
     const bool whole_item = i0 == 0 && i1 == rg.tiles;
     const int64_t piece = 2 * (int64_t)blockIdx.x + (i0 == 0);
@@ -340,40 +437,59 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM<D>) k_attn_rows(Args a)
 // Joins the pieces of the items that cross blocks: grid (blocks of the first kernel, RB), one row per block; desc[c] =
 // (sequence, item, last block, rows) when block c holds an item's first piece. Its pieces are slot 2c + 1 and the even
 // slots of the blocks after c, summed in that order.
+constexpr int JOIN_T = 256;
 template <typename E, int D, int ROWS>
-__global__ void __launch_bounds__(128) k_attn_join(Args a) {
+__global__ void __launch_bounds__(JOIN_T) k_attn_join(Args a) {
   pdl_wait();
   const int4 d = a.desc[blockIdx.x];
   const int r = blockIdx.y;
   if (d.x < 0 || r >= d.w) return;
-  constexpr int LANES = D / 4, G = 128 / LANES;       // threads of a row, groups that share the pieces
+  constexpr int LANES = D / 4, G = JOIN_T / LANES;    // threads of a row, groups that share the pieces
   __shared__ float4 part[G][LANES];
-  __shared__ float2 pml[G];
-  const int c0 = blockIdx.x, n = d.z - c0 + 1, c = threadIdx.x % LANES, g = threadIdx.x / LANES;
+  __shared__ float factor[JOIN_T], warp_m[JOIN_T / 32], warp_l[JOIN_T / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int c0 = blockIdx.x, n = d.z - c0 + 1, c = tid % LANES, g = tid / LANES;
   auto slot = [&](int i) { return (i == 0 ? 2 * (int64_t)c0 + 1 : 2 * (int64_t)(c0 + i)) * ROWS + r; };
   float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, a.ml[slot(i)].x);
+  for (int i = tid; i < n; i += JOIN_T) m = fmaxf(m, a.ml[slot(i)].x);
+  m = warp_max(m);
+  if (lane == 0) warp_m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_T / 32; ++w) m = fmaxf(m, warp_m[w]);
   const float u = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = g; i < n; i += G) {
-    const float2 e = a.ml[slot(i)];
-    const float f = ex2(e.x - u);
-    const float4 x = *(const float4*)(a.acc + slot(i) * D + c * 4);
-    l += e.y * f;
-    o.x += x.x * f;
-    o.y += x.y * f;
-    o.z += x.z * f;
-    o.w += x.w * f;
+  for (int i0 = 0; i0 < n; i0 += JOIN_T) {
+    __syncthreads();
+    if (i0 + tid < n) {
+      const float2 e = a.ml[slot(i0 + tid)];
+      factor[tid] = ex2(e.x - u);
+      l += e.y * factor[tid];
+    }
+    __syncthreads();
+    const int k = min(n - i0, JOIN_T);
+#pragma unroll 8
+    for (int i = g; i < k; i += G) {
+      const float f = factor[i];
+      const float4 x = *(const float4*)(a.acc + slot(i0 + i) * D + c * 4);
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
+    }
   }
+  l = warp_sum(l);
+  if (lane == 0) warp_l[warp] = l;
   part[g][c] = o;
-  if (c == 0) pml[g] = make_float2(l, 0.f);
   __syncthreads();
   if (g) return;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < JOIN_T / 32; ++w) l += warp_l[w];
+#pragma unroll
   for (int x = 1; x < G; ++x) {
     const float4 y = part[x][c];
-    l += pml[x].x;
     o.x += y.x;
     o.y += y.y;
     o.z += y.z;
@@ -388,14 +504,7 @@ __global__ void __launch_bounds__(128) k_attn_join(Args a) {
   if (a.lse && c == 0) a.lse[row] = (m + log2f(l)) * LN2;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
-int blocks_of(int dim) { return sm_count() * (dim == 256 ? BLOCKS_PER_SM<256> : BLOCKS_PER_SM<128>); }
+int row_blocks() { return ssb_sm_count() * BLOCKS_PER_SM; }
 
 struct Layout {
   int64_t desc, ml, acc, bytes;
@@ -409,30 +518,28 @@ Layout layout_of(int blocks, int rows, int dim) {
   return l;
 }
 
-template <typename E, int D>
+template <typename E, int D, int RB>
 int launch_rows(Args& a, uint8_t* ws, cudaStream_t stream) {
-  const int blocks = blocks_of(D);
+  const int blocks = row_blocks();
   const Layout l = layout_of(blocks, RB, D);
   a.desc = (int4*)(ws + l.desc);
   a.ml = (float2*)(ws + l.ml);
   a.acc = (float*)(ws + l.acc);
-  auto kern = k_attn_rows<E, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM<D>);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return (int)e;
-  }
-  ssb_note_smem("attn_decode", kern, SMEM<D>);
-  int rc = ssb_launch(kern, dim3(blocks), dim3(NW * 32), SMEM<D>, stream, false, a);
+  auto kern = k_attn_rows<E, D, RB>;
+  static std::atomic<uint64_t> done{0};
+  int rc = ssb_setup_kernel(done, "attn_decode", kern, SMEM<D, RB>);
   if (rc) return rc;
-  return ssb_launch(k_attn_join<E, D, RB>, dim3(blocks, RB), dim3(128), 0, stream, true, a);
+  rc = ssb_launch(kern, dim3(blocks), dim3(NW * 32), SMEM<D, RB>, stream, false, a);
+  if (rc) return rc;
+  return ssb_launch(k_attn_join<E, D, RB>, dim3(blocks, RB), dim3(JOIN_T), 0, stream, true, a);
 }
 
+// Items of 8 rows where that holds every row of a key head, else of 16: the second 8 cost registers and instructions.
 template <typename E>
-int launch_dim(Args& a, int dim, uint8_t* ws, cudaStream_t st) {
-  if (dim == 64) return launch_rows<E, 64>(a, ws, st);
-  if (dim == 128) return launch_rows<E, 128>(a, ws, st);
-  return launch_rows<E, 256>(a, ws, st);
+int launch_dim(Args& a, int dim, bool few, uint8_t* ws, cudaStream_t st) {
+  if (dim == 64) return few ? launch_rows<E, 64, 8>(a, ws, st) : launch_rows<E, 64, 16>(a, ws, st);
+  if (dim == 128) return few ? launch_rows<E, 128, 8>(a, ws, st) : launch_rows<E, 128, 16>(a, ws, st);
+  return few ? launch_rows<E, 256, 8>(a, ws, st) : launch_rows<E, 256, 16>(a, ws, st);
 }
 
 // t / d = (mulhi(t, mul) + t) >> shift for t < 2^31 (round-up reciprocal of a 32-bit division).
@@ -490,7 +597,7 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
 using namespace attn;
 
 static int64_t workspace(int dim, int n, int64_t rows, int heads, int kv_heads, bool prefill) {
-  return prefill ? prefill_workspace(dim, n, rows, heads, kv_heads) : layout_of(blocks_of(dim), RB, dim).bytes;
+  return prefill ? prefill_workspace(dim, n, rows, heads, kv_heads) : layout_of(row_blocks(), 16, dim).bytes;
 }
 
 extern "C" int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads,
@@ -517,14 +624,15 @@ extern "C" int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stri
   if ((int64_t)q_len * (heads / kv_heads) > 128) return SSB_EUNSUPPORTED;
   if (n == 0 || q_len == 0) return SSB_OK;
   SSB_CHECK_ARG(q && k && v && table && lengths && out && ws);
-  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= layout_of(blocks_of(dim), RB, dim).bytes);
+  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= layout_of(row_blocks(), 16, dim).bytes);
   a.q_seq = q_seq_stride;
   a.q_tok = q_tok_stride;
   a.q_head = q_head_stride;
   a.q_len = q_len;
   a.rows = (int64_t)n * q_len;
-  return q_type == SSB_BF16 ? launch_dim<__nv_bfloat16>(a, dim, (uint8_t*)ws, (cudaStream_t)stream)
-                            : launch_dim<__half>(a, dim, (uint8_t*)ws, (cudaStream_t)stream);
+  const bool few = q_len * a.group <= 8;
+  return q_type == SSB_BF16 ? launch_dim<__nv_bfloat16>(a, dim, few, (uint8_t*)ws, (cudaStream_t)stream)
+                            : launch_dim<__half>(a, dim, few, (uint8_t*)ws, (cudaStream_t)stream);
 }
 
 extern "C" int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_stride, int64_t q_head_stride,

@@ -154,6 +154,8 @@ template <int MB, int T>
 __global__ void __launch_bounds__(PLAN_T) k_prefill_plan(Args a, Work w, int blocks) {
   __shared__ int part[33];
   __shared__ long long lpart[33];
+  pdl_wait();
+  pdl_trigger();
   int items = 0;
   for (int b0 = 0; b0 < a.n; b0 += PLAN_T) {
     const int b = b0 + threadIdx.x;
@@ -377,6 +379,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     fence_mbar_init();
   }
   pdl_wait();
+  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -781,20 +784,13 @@ __global__ void __launch_bounds__(2 * D) k_prefill_join(Args a, Work w) {
   if (a.lse && c == 0) a.lse[row] = (m + log2f(l)) * LN2;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 struct Layout {
   int64_t item0, ctl, units, joints, ml, acc, bytes;
   int max_units, max_slots;
 };
 int64_t up(int64_t x) { return (x + 127) / 128 * 128; }
 Layout layout_of(int dim, int n, int64_t rows, int heads, int kv_heads) {
-  const int mb = dim == 256 ? 128 : 256, blocks = sm_count();
+  const int mb = dim == 256 ? 128 : 256, blocks = ssb_sm_count();
   Layout l;
   const int64_t items = (rows * (heads / kv_heads) / mb + n) * kv_heads;
   l.max_slots = 4 * blocks;
@@ -868,16 +864,13 @@ int launch(Args& a, uint8_t* ws, const Layout& l, cudaStream_t stream) {
   a.ml = (float2*)(ws + l.ml);
   a.acc = (float*)(ws + l.acc);
   auto kern = k_prefill<E, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return (int)e;
-  }
-  ssb_note_smem("attn_prefill", kern, C::SMEM);
+  static std::atomic<uint64_t> done{0};
+  int rc = ssb_setup_kernel(done, "attn_prefill", kern, C::SMEM);
+  if (rc) return rc;
   Maps maps = {};
   make_maps(maps, w, a, sizeof(E) == 2 && idesc_of<E>(128, 64, false) == idesc_of<__nv_bfloat16>(128, 64, false), D, C::T);
-  const int blocks = sm_count();
-  int rc = ssb_launch(k_prefill_plan<C::MB, C::T>, dim3(1), dim3(PLAN_T), 0, stream, false, a, w, blocks);
+  const int blocks = ssb_sm_count();
+  rc = ssb_launch(k_prefill_plan<C::MB, C::T>, dim3(1), dim3(PLAN_T), 0, stream, false, a, w, blocks);
   if (rc) return rc;
   rc = ssb_launch(kern, dim3(blocks), dim3(C::THREADS), C::SMEM, stream, true, maps, a, w);
   if (rc) return rc;

@@ -24,6 +24,22 @@ void ssb_note_smem_bytes(const char* name, int bytes) {
   table()[name] = bytes;
 }
 
+int ssb_sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
 extern "C" int ssb_kernel_smem(const char* name) {
   if (!name) return -1;
   std::lock_guard<std::mutex> g(g_mu);

@@ -130,8 +130,15 @@ def ptr(t):
     return t.data_ptr()
 
 
+# torch.cuda.current_stream() builds a Stream object (about 3 us of host time a call); the handle alone is enough here.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device_index = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None or _device_index is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_device_index())
 
 
 _NAMES = {SSB_EINVAL: "SSB_EINVAL (bad argument)", SSB_EUNSUPPORTED: "SSB_EUNSUPPORTED (shape not handled)",

@@ -66,7 +66,7 @@ def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window
         raise ValueError("err must be one int32")
     shape = q.shape
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous, with q's shape and type")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:-1] or not lse.is_contiguous()):
