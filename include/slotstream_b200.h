@@ -493,15 +493,16 @@ int ssb_kv_compact(const ssb_kv_cache* c, void* stream);
  * (nullable) maps batch row b to its table row, one of table_rows (others read as empty and set
  * SSB_ERR_SEQUENCE). What no query of the call sees is not read; a visible token whose
  * table entry lies outside [0, pages) reads as zeros and sets SSB_ERR_PAGE_RANGE. heads is a multiple of kv_heads,
- * query head h reads key head h / (heads / kv_heads); dim 64, 128 or 256; scale positive and finite. ws: workspace of ssb_attn_workspace bytes,
- * contents irrelevant between calls; calls sharing it must not overlap.
+ * query head h reads key head h / (heads / kv_heads); dim 64, 128 or 256; scale positive and finite. ws: workspace of ssb_attn_workspace bytes for
+ * the call's sizes (rows = all query tokens; 0: ws may be NULL), contents irrelevant between calls; calls sharing it must
+ * not overlap.
  *
  * ssb_attn_decode: q [n, q_len, heads, dim] (strides in elements, multiples of 8), the q_len newest tokens of each
  * sequence (positions lengths - q_len ..; a position below 0 has no visible token). q_len * heads / kv_heads <= 128.
  * ssb_attn_prefill: ragged q [rows, heads, dim]; rows starts[b] <= r < starts[b + 1] are the newest tokens of
  * sequence b. out / lse are contiguous. */
-int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads, int32_t prefill,
-                       int64_t* bytes);
+int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads, int32_t page_size,
+                       int32_t max_pages, int32_t window, int32_t sinks, int32_t prefill, int64_t* bytes);
 int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride,
                     const void* k, const void* v, int64_t page_stride, int64_t head_stride, int64_t token_stride,
                     int32_t n, int32_t q_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t page_size,

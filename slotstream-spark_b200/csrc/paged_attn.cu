@@ -7,13 +7,15 @@
 // would otherwise take more issue slots than the loads leave; tcgen05's 128-row tiles would be mostly padding here. The
 // products are taken transposed -- S^T = K Q^T, O^T = V^T P^T -- so that the query rows are the instruction's 8 columns
 // and nothing is padded to 16 for groups of up to eight rows (at 131,072 tokens and head size 256, 84 us with rows padded to
-// 16, REPLACE us now).
+// 16, 57 us now).
 //
 // A block has NW warps that work alone: each walks every NW-th sub-tile of TW tokens through its own ring of cp.async
 // units (no block barrier inside an item), and the warps' (max, sum, accumulator) are joined through shared
 // memory at the end of the item. p is rounded to the inputs' type for the second product (relative 2^-8 for bf16,
 // 2^-11 for fp16, as the library's other tensor-core inputs); its sum is taken before the rounding, in fp32.
 #include "paged_attn.cuh"
+
+#include <cooperative_groups.h>
 
 #include "affine.cuh"
 #include "tc_common.cuh"
@@ -74,8 +76,8 @@ template <int D, int RB>
 constexpr int SMEM = RB * D * 2 + NW * NU<D> * UNIT<D>;
 constexpr int BLOCKS_PER_SM = 2;
 
-template <typename E, int D, int RB>
-__global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
+template <typename E, int D, int RB, bool DIRECT>
+__global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a, int cluster) {
   constexpr int T = NW * TW<D>, CPR = D / 8, NB = RB / 8;       // tokens of a tile, 16-byte chunks and blocks of 8 rows
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long scan[NW];
@@ -91,7 +93,8 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
   auto weight_of = [&](int b) -> long long {
     if (b >= a.n) return 0;
     const Seq s = seq_of(a, b);
-    return (long long)a.kv_heads * ((s.q * a.group + RB - 1) / RB) * range_of(a, s.len - s.q, s.len - 1, T).tiles;
+    const long long items = (long long)a.kv_heads * ((s.q * a.group + RB - 1) / RB);
+    return DIRECT ? items : items * range_of(a, s.len - s.q, s.len - 1, T).tiles;
   };
   auto scan_block = [&](long long w, long long* sum) {      // inclusive
     long long inc = w;
@@ -112,7 +115,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
     *sum = all;
     return before + inc;
   };
-  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (!DIRECT && tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
   long long w0 = weight_of(tid), total;
   const long long inc0 = scan_block(w0, &total);
   const long long first_total = total;
@@ -123,8 +126,10 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
     scan_block(more, &rest);
     total += rest;
   }
-  const long long chunk = max((total + gridDim.x - 1) / gridDim.x, 1ll);
-  const long long lo = chunk * blockIdx.x, hi = min(lo + chunk, total);
+  // DIRECT: an item a cluster, whose blocks share its tiles (all of a cluster returns here, or none does)
+  const int rank = DIRECT ? blockIdx.x % cluster : 0;
+  const long long chunk = DIRECT ? 1 : max((total + gridDim.x - 1) / gridDim.x, 1ll);
+  const long long lo = DIRECT ? blockIdx.x / cluster : chunk * blockIdx.x, hi = min(lo + chunk, total);
   if (lo >= hi) return;
   // the sequence that holds tile `lo`, and its first tile
   if (lo >= inc0 - w0 && lo < inc0) {
@@ -150,30 +155,19 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
   while (at < hi) {
     const Range rg = range_of(a, s.len - s.q, s.len - 1, T);
     const int nb = (s.q * a.group + RB - 1) / RB;
-    const long long weight = (long long)a.kv_heads * nb * rg.tiles;
+    const long long unit = DIRECT ? 1 : rg.tiles, weight = a.kv_heads * nb * unit;
     if (at >= begin + weight) {
       begin += weight;
       s = seq_of(a, ++b);
       continue;
     }
     // ---- one item, or the part of it inside this block
-    const int item = (int)((at - begin) / rg.tiles), h = item / nb, rb = item - h * nb;
-    const long long item0 = begin + (long long)item * rg.tiles;
-    const int i0 = (int)(at - item0), i1 = (int)min((long long)rg.tiles, hi - item0);
+    const int item = (int)((at - begin) / unit), h = item / nb, rb = item - h * nb;
+    const long long item0 = begin + item * unit;
+    const int i0 = DIRECT ? (int)((long long)rg.tiles * rank / cluster) : (int)(at - item0);
+    const int i1 = DIRECT ? (int)((long long)rg.tiles * (rank + 1) / cluster) : (int)min((long long)rg.tiles, hi - item0);
     const int r0 = rb * RB, rows = min(RB, s.q * a.group - r0);
     const int p_first = s.len - s.q, p_lo = p_first + r0 / a.group, p_hi = p_first + (r0 + rows - 1) / a.group;
-
-    for (int i = tid; i < RB * CPR; i += NW * 32) {
-      const int r = i / CPR, c = i - r * CPR;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int t = (r0 + r) / a.group, g = (r0 + r) - t * a.group;
-        const int64_t qt = a.starts ? (s.q0 + t) * a.q_tok : (int64_t)b * a.q_seq + t * a.q_tok;
-        v = __ldg((const uint4*)(a.q + qt + (h * a.group + g) * a.q_head + c * 8));
-      }
-      *(uint4*)(sq + swz<D>(r, c)) = v;
-    }
-    __syncthreads();
 
     const uint16_t *kh = a.k + h * a.sh, *vh = a.v + h * a.sh;
     const int32_t* trow = a.table + (int64_t)max(s.row, 0) * a.max_pages;
@@ -209,6 +203,20 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
       asm volatile("cp.async.wait_group %0;" ::"n"(NU<D> - 2) : "memory");
       __syncwarp();
     };
+
+#pragma unroll
+    for (int n = 0; n < NU<D> - 1; ++n) issue(n);
+    for (int i = tid; i < RB * CPR; i += NW * 32) {
+      const int r = i / CPR, c = i - r * CPR;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int t = (r0 + r) / a.group, g = (r0 + r) - t * a.group;
+        const int64_t qt = a.starts ? (s.q0 + t) * a.q_tok : (int64_t)b * a.q_seq + t * a.q_tok;
+        v = __ldg((const uint4*)(a.q + qt + (h * a.group + g) * a.q_head + c * 8));
+      }
+      *(uint4*)(sq + swz<D>(r, c)) = v;
+    }
+    __syncthreads();
 
     // Rows are the columns of both products (see the top): a thread holds rows 8 n + 2 (lane % 4) and the next of every
     // n < NB, as columns of S^T (tokens lane / 4 and + 8 of a group of 16) and of O^T (dims lane / 4 and + 8 of 16).
@@ -248,8 +256,6 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
         }
     }
 
-#pragma unroll
-    for (int n = 0; n < NU<D> - 1; ++n) issue(n);
     for (int i = i0; i < i1; ++i) {
       const int un = 2 * (i - i0);
       landed();
@@ -379,7 +385,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
     __syncthreads();
     float* wacc = (float*)(smem + RB * D * 2);                         // [NW][RB][D]
     float2* wml = (float2*)(wacc + NW * RB * D);                        // [NW][RB]
-    static_assert(NW * RB * D * 4 + NW * RB * 8 <= NW * NU<D> * UNIT<D>, "the join needs the ring");
+    static_assert((NW + 1) * RB * (D * 4 + 8) <= NW * NU<D> * UNIT<D>, "the join needs the ring");
 #pragma unroll
     for (int j = 0; j < KS; ++j)
 #pragma unroll
@@ -393,8 +399,17 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) wml[warp * RB + n * 8 + lane * 2 + y] = make_float2(m[n][y], l[n][y]);
     __syncthreads();
-    const bool whole_item = i0 == 0 && i1 == rg.tiles;
+    const bool whole_item = DIRECT ? cluster == 1 : i0 == 0 && i1 == rg.tiles;
     const int64_t piece = 2 * (int64_t)blockIdx.x + (i0 == 0);
+    float* macc = (float*)(wml + NW * RB);                               // [RB][D], of this block (DIRECT)
+    float2* mml = (float2*)(macc + RB * D);                              // [RB]
+    auto finish = [&](int r, int c, float4 o, float m, float l) {
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const int t = (r0 + r) / a.group, g = (r0 + r) - t * a.group;
+      const int64_t row = (s.q0 + t) * a.heads + h * a.group + g;
+      *(uint2*)(a.out + row * D + c) = make_uint2(pack2<E>(o.x * inv, o.y * inv), pack2<E>(o.z * inv, o.w * inv));
+      if (a.lse && c == 0) a.lse[row] = (m + log2f(l)) * LN2;
+    };
     for (int i = tid; i < rows * (D / 4); i += NW * 32) {
       const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
       float m = -INFINITY, l = 0.f;
@@ -414,21 +429,44 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a) {
         o.w += x.w * f;
       }
       if (whole_item) {
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        const int t = (r0 + r) / a.group, g = (r0 + r) - t * a.group;
-        const int64_t row = (s.q0 + t) * a.heads + h * a.group + g;
-        *(uint2*)(a.out + row * D + c) = make_uint2(pack2<E>(o.x * inv, o.y * inv), pack2<E>(o.z * inv, o.w * inv));
-        if (a.lse && c == 0) a.lse[row] = (m + log2f(l)) * LN2;
+        finish(r, c, o, m, l);
+      } else if (DIRECT) {
+        *(float4*)(macc + r * D + c) = o;
+        if (c == 0) mml[r] = make_float2(m, l);
       } else {
         *(float4*)(a.acc + (piece * RB + r) * D + c) = o;
         if (c == 0) a.ml[piece * RB + r] = make_float2(m, l);
       }
     }
+    if (DIRECT && cluster > 1) {                     // join the cluster's blocks through their shared memory, in rank order
+      cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+      cl.sync();
+      for (int i = tid * cluster + rank; i < rows * (D / 4); i += NW * 32 * cluster) {
+        const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < cluster; ++k) m = fmaxf(m, cl.map_shared_rank(mml, k)[r].x);
+        const float u = m == -INFINITY ? 0.f : m;
+        for (int k = 0; k < cluster; ++k) {
+          const float2 e = cl.map_shared_rank(mml, k)[r];
+          const float f = ex2(e.x - u);
+          const float4 x = *(const float4*)(cl.map_shared_rank(macc, k) + r * D + c);
+          l += e.y * f;
+          o.x += x.x * f;
+          o.y += x.y * f;
+          o.z += x.z * f;
+          o.w += x.w * f;
+        }
+        finish(r, c, o, m, l);
+      }
+      cl.sync();                                     // nobody leaves while another reads its memory
+    }
     if (tid == 0) {
       if (s.row < 0) set_err(a.err, SSB_ERR_SEQUENCE);
-      if (i0 == 0 && !whole_item)
+      if (!DIRECT && i0 == 0 && !whole_item)
         a.desc[blockIdx.x] = make_int4(b, item, (int)((item0 + rg.tiles - 1) / chunk), rows);
     }
+    if (DIRECT) return;
     __syncthreads();
     at = item0 + i1;
   }
@@ -518,28 +556,103 @@ Layout layout_of(int blocks, int rows, int dim) {
   return l;
 }
 
+// Blocks that share an item when each item is taken whole in one launch (0: all tiles split evenly over the GPU, joined by a
+// second launch). That saves the second launch and the pieces' way through memory, at the price of an uneven split, so it is
+// for items of few tiles, counted from the longest sequence that the table (or the window) allows: clusters grow until a block
+// has at most DIRECT_GOOD tiles or the GPU is full; more than DIRECT_MOST tiles a block, or more than DIRECT_WAVES fillings
+// of the GPU, go the other way. Device time, whole items against split (16 heads, 2 key heads, head size 256): 16 sequences of
+// 1,000 tokens 12.8 against 13.9 us, 64 of 500 19.7 against 22.7, one of 2,000 12.5 against 11.2 (but one launch less, 4 us
+// of host time); 24 heads, 8 key heads, head size 64, 256 sequences of 500: 70 against 59.
+constexpr int DIRECT_GOOD = 4, DIRECT_MOST = 8, DIRECT_WAVES = 4;
+int tiles_at_most(const Args& a, int tile) {
+  int64_t len = (int64_t)a.max_pages * a.page_size;
+  if (a.window) {
+    const int64_t q = a.starts ? a.rows : a.q_len, seen = (int64_t)a.window + q + a.sinks + 2 * tile;
+    len = len < seen ? len : seen;
+  }
+  return (int)((len + tile - 1) / tile);
+}
+int direct_cluster(int tiles, int64_t items) {
+  int c = 1;
+  while (c < 8 && tiles > DIRECT_GOOD * c && items * 2 * c <= row_blocks()) c *= 2;
+  return tiles > DIRECT_MOST * c || items * c > (int64_t)DIRECT_WAVES * row_blocks() ? 0 : c;
+}
+int64_t items_of(const Args& a, int rb) {
+  return a.starts ? (a.rows * a.group / rb + a.n) * a.kv_heads
+                  : (int64_t)a.n * a.kv_heads * ((a.q_len * a.group + rb - 1) / rb);
+}
+constexpr int tile_of(int dim) { return NW * (dim == 64 ? TW<64> : dim == 128 ? TW<128> : TW<256>); }
+
+// Items of 8 rows where that holds every row of a key head, else of 16: the second 8 cost registers and instructions.
+int rows_per_item(const Args& a) { return a.q_len * a.group <= 8 && !a.starts ? 8 : 16; }
+
+// Prompts go to this kernel too where it takes every item whole and the call is at most SMALL_TILES tiles a block: the
+// tcgen05 kernel's plan, tensor maps and 128-row tiles cost more there. Device time, this one against that one: 5 ragged
+// prompts of up to 129 tokens (8 heads, 2 key heads, size 64) 7.7 against 20.4 us; one of 256 tokens (32 heads, 8 key heads,
+// size 128; 5 tiles a block) 20.9 against 25.3; one of 512 (17 tiles a block) 55 against 37.
+constexpr int SMALL_TILES = 8;
+bool small_prompt(const Args& a, int dim) {
+  const int tiles = tiles_at_most(a, tile_of(dim));
+  const int64_t items = items_of(a, 16);
+  return direct_cluster(tiles, items) && items * tiles <= (int64_t)SMALL_TILES * row_blocks();
+}
+
+int64_t workspace(const Args& a, int dim) {
+  if (a.starts && !small_prompt(a, dim)) return prefill_workspace(dim, a.n, a.rows, a.heads, a.kv_heads);
+  const int rb = rows_per_item(a);
+  return direct_cluster(tiles_at_most(a, tile_of(dim)), items_of(a, rb)) ? 0 : layout_of(row_blocks(), rb, dim).bytes;
+}
+
 template <typename E, int D, int RB>
 int launch_rows(Args& a, uint8_t* ws, cudaStream_t stream) {
+  const int64_t items = items_of(a, RB);
+  if (const int c = direct_cluster(tiles_at_most(a, NW * TW<D>), items)) {
+    auto kern = k_attn_rows<E, D, RB, true>;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = ssb_setup_kernel(done, "attn_decode", kern, SMEM<D, RB>)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * c));
+    cfg.blockDim = dim3(NW * 32);
+    cfg.dynamicSmemBytes = SMEM<D, RB>;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, c);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return (int)e;
+  }
   const int blocks = row_blocks();
   const Layout l = layout_of(blocks, RB, D);
   a.desc = (int4*)(ws + l.desc);
   a.ml = (float2*)(ws + l.ml);
   a.acc = (float*)(ws + l.acc);
-  auto kern = k_attn_rows<E, D, RB>;
+  auto kern = k_attn_rows<E, D, RB, false>;
   static std::atomic<uint64_t> done{0};
   int rc = ssb_setup_kernel(done, "attn_decode", kern, SMEM<D, RB>);
   if (rc) return rc;
-  rc = ssb_launch(kern, dim3(blocks), dim3(NW * 32), SMEM<D, RB>, stream, false, a);
+  rc = ssb_launch(kern, dim3(blocks), dim3(NW * 32), SMEM<D, RB>, stream, false, a, 1);
   if (rc) return rc;
   return ssb_launch(k_attn_join<E, D, RB>, dim3(blocks, RB), dim3(JOIN_T), 0, stream, true, a);
 }
 
-// Items of 8 rows where that holds every row of a key head, else of 16: the second 8 cost registers and instructions.
 template <typename E>
-int launch_dim(Args& a, int dim, bool few, uint8_t* ws, cudaStream_t st) {
+int launch_dim(Args& a, int dim, uint8_t* ws, cudaStream_t st) {
+  const bool few = rows_per_item(a) == 8;
   if (dim == 64) return few ? launch_rows<E, 64, 8>(a, ws, st) : launch_rows<E, 64, 16>(a, ws, st);
   if (dim == 128) return few ? launch_rows<E, 128, 8>(a, ws, st) : launch_rows<E, 128, 16>(a, ws, st);
   return few ? launch_rows<E, 256, 8>(a, ws, st) : launch_rows<E, 256, 16>(a, ws, st);
+}
+
+int launch_checked(Args& a, int dim, bool bf16, void* ws, int64_t ws_bytes, void* stream) {
+  const int64_t need = workspace(a, dim);
+  SSB_CHECK_ARG(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need));
+  if (a.starts && !small_prompt(a, dim)) return prefill_launch(a, dim, bf16, ws, stream);
+  return bf16 ? launch_dim<__nv_bfloat16>(a, dim, (uint8_t*)ws, (cudaStream_t)stream)
+              : launch_dim<__half>(a, dim, (uint8_t*)ws, (cudaStream_t)stream);
 }
 
 // t / d = (mulhi(t, mul) + t) >> shift for t < 2^31 (round-up reciprocal of a 32-bit division).
@@ -596,16 +709,27 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
 
 using namespace attn;
 
-static int64_t workspace(int dim, int n, int64_t rows, int heads, int kv_heads, bool prefill) {
-  return prefill ? prefill_workspace(dim, n, rows, heads, kv_heads) : layout_of(row_blocks(), 16, dim).bytes;
-}
-
 extern "C" int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads,
-                                  int32_t prefill, int64_t* bytes) {
+                                  int32_t page_size, int32_t max_pages, int32_t window, int32_t sinks, int32_t prefill,
+                                  int64_t* bytes) {
   SSB_CHECK_ARG(bytes && n >= 0 && rows >= 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0);
-  SSB_CHECK_ARG(rows * (heads / kv_heads) < (1ll << 30));
+  SSB_CHECK_ARG(rows * (heads / kv_heads) < (1ll << 30) && page_size > 0 && max_pages > 0 && window >= 0 && sinks >= 0);
   if (dim != 64 && dim != 128 && dim != 256) return SSB_EUNSUPPORTED;
-  *bytes = workspace(dim, n, rows, heads, kv_heads, prefill != 0);
+  if (!prefill && n && rows % n) return SSB_EINVAL;
+  Args a = {};
+  a.n = n;
+  a.rows = rows;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.window = window;
+  a.sinks = window ? sinks : 0;
+  const int32_t some = 0;
+  if (prefill) a.starts = &some;                     // only whether there are any matters here
+  else a.q_len = n ? (int32_t)(rows / n) : 0;
+  *bytes = n && rows ? workspace(a, dim) : 0;
   return SSB_OK;
 }
 
@@ -623,16 +747,13 @@ extern "C" int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stri
   SSB_CHECK_ARG(q_len >= 0 && (q_seq_stride | q_tok_stride | q_head_stride) % 8 == 0);
   if ((int64_t)q_len * (heads / kv_heads) > 128) return SSB_EUNSUPPORTED;
   if (n == 0 || q_len == 0) return SSB_OK;
-  SSB_CHECK_ARG(q && k && v && table && lengths && out && ws);
-  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= layout_of(row_blocks(), 16, dim).bytes);
+  SSB_CHECK_ARG(q && k && v && table && lengths && out);
   a.q_seq = q_seq_stride;
   a.q_tok = q_tok_stride;
   a.q_head = q_head_stride;
   a.q_len = q_len;
   a.rows = (int64_t)n * q_len;
-  const bool few = q_len * a.group <= 8;
-  return q_type == SSB_BF16 ? launch_dim<__nv_bfloat16>(a, dim, few, (uint8_t*)ws, (cudaStream_t)stream)
-                            : launch_dim<__half>(a, dim, few, (uint8_t*)ws, (cudaStream_t)stream);
+  return launch_checked(a, dim, q_type == SSB_BF16, ws, ws_bytes, stream);
 }
 
 extern "C" int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_stride, int64_t q_head_stride,
@@ -648,11 +769,10 @@ extern "C" int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_str
     return rc;
   SSB_CHECK_ARG(rows >= 0 && rows * (heads / kv_heads) < (1ll << 30) && (q_tok_stride | q_head_stride) % 8 == 0);
   if (n == 0 || rows == 0) return SSB_OK;
-  SSB_CHECK_ARG(q && k && v && table && lengths && starts && out && ws);
-  SSB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_bytes >= workspace(dim, n, rows, heads, kv_heads, true));
+  SSB_CHECK_ARG(q && k && v && table && lengths && starts && out);
   a.q_tok = q_tok_stride;
   a.q_head = q_head_stride;
   a.starts = starts;
   a.rows = rows;
-  return prefill_launch(a, dim, q_type == SSB_BF16, ws, stream);
+  return launch_checked(a, dim, q_type == SSB_BF16, ws, ws_bytes, stream);
 }

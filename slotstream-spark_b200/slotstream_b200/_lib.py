@@ -91,7 +91,7 @@ SIGNATURES = {
     "ssb_kv_fork": [_P, _P, _P, _I32, _P],
     "ssb_kv_free": [_P, _P, _P, _P, _I32, _P],
     "ssb_kv_compact": [_P, _P],
-    "ssb_attn_workspace": [_I32, _I32, _I64, _I32, _I32, _I32, _P],
+    "ssb_attn_workspace": [_I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "ssb_attn_decode": [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
                         _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
     "ssb_attn_prefill": [_P, _I32, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32,
@@ -135,10 +135,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device_index = getattr(torch._C, "_cuda_getDevice", None)
 
 
+def device_index():
+    return torch.cuda.current_device() if _device_index is None else _device_index()
+
+
 def stream():
-    if _raw_stream is None or _device_index is None:
+    if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
-    return _raw_stream(_device_index())
+    return _raw_stream(device_index())
 
 
 _NAMES = {SSB_EINVAL: "SSB_EINVAL (bad argument)", SSB_EUNSUPPORTED: "SSB_EUNSUPPORTED (shape not handled)",

@@ -23,34 +23,43 @@ _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _WS = {}
 
 
-def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, kv_heads: int, prefill: bool = False) -> int:
-    """Bytes of ``ws`` for ``n`` sequences with ``rows`` query tokens in all."""
-    key = (head_dim, n, rows, heads, kv_heads, prefill, torch.cuda.current_device())
+def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, kv_heads: int, page_size: int, max_pages: int,
+                    window: int = 0, sinks: int = 0, prefill: bool = False) -> int:
+    """Bytes of ``ws`` for ``n`` sequences with ``rows`` query tokens in all (0: none is needed). Small calls need none."""
+    key = (head_dim, n, rows, heads, kv_heads, page_size, max_pages, window, sinks, prefill, _lib.device_index())
     got = _WS.get(key)
     if got is None:
         b = ctypes.c_int64()
-        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, rows, heads, kv_heads, int(prefill), ctypes.byref(b)),
-                   "attention workspace")
+        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, rows, heads, kv_heads, page_size, max_pages, window, sinks,
+                                                 int(prefill), ctypes.byref(b)), "attention workspace")
         if len(_WS) > 4096:
             _WS.clear()
         got = _WS[key] = b.value
     return got
 
 
-def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out, lse):
-    tag = _TYPES.get(q.dtype)
-    if tag is None or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
-        raise ValueError("q, k_pages and v_pages must all be bf16 or all fp16")
+def _bad_pages(q, k_pages, v_pages, dim, heads):
+    """The refusal for the cache's views (built only when one of the checks in the calls below fails)."""
+    if q.dtype not in _TYPES or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        return ValueError("q, k_pages and v_pages must all be bf16 or all fp16")
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != dim:
-        raise ValueError(f"k_pages and v_pages must both be [pages, kv_heads, page_size, {dim}]")
-    ks = k_pages.stride()
-    if ks != v_pages.stride() or ks[3] != 1:
-        raise ValueError("k_pages and v_pages must have the same strides, the last one 1")
-    if heads % k_pages.shape[1]:
-        raise ValueError(f"{heads} query heads are no multiple of {k_pages.shape[1]} key heads")
+        return ValueError(f"k_pages and v_pages must both be [pages, kv_heads, page_size, {dim}]")
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        return ValueError("k_pages and v_pages must have the same strides, the last one 1")
+    return ValueError(f"{heads} query heads are no multiple of {k_pages.shape[1]} key heads")
+
+
+def _attend(call, what, q, heads, dim, n, tokens, starts, q_args, k_pages, v_pages, page_table, lengths, out, lse, scale,
+            window, sinks, ids, err, ws):
+    """The checks, allocations and arguments that both entry points share."""
+    tag = _TYPES.get(q.dtype)
+    ps, ks = k_pages.shape, k_pages.stride()
+    if tag is None or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype or len(ps) != 4 or v_pages.shape != ps \
+            or v_pages.stride() != ks or ks[3] != 1 or ps[3] != dim or heads % ps[1]:
+        raise _bad_pages(q, k_pages, v_pages, dim, heads)
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
         raise ValueError("page_table must be a contiguous int32 [rows, max_pages]")
-    rows = page_table.shape[0]
+    rows, max_pages = page_table.shape
     if lengths.dtype != torch.int32 or lengths.shape != (rows,) or not lengths.is_contiguous():
         raise ValueError("lengths must be a contiguous int32 vector, one per row of page_table")
     if ids is not None:
@@ -60,7 +69,9 @@ def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window
         raise ValueError(f"{n} sequences, but page_table has {rows} rows")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    if scale is not None and not 0 < scale < math.inf:
+    if scale is None:
+        scale = dim ** -0.5
+    elif not 0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
     if err is not None and (err.dtype != torch.int32 or err.numel() != 1):
         raise ValueError("err must be one int32")
@@ -71,16 +82,20 @@ def _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window
         raise ValueError("out must be contiguous, with q's shape and type")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:-1] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous fp32 tensor of q's shape without the last dimension")
-    return tag, ks, rows, out
-
-
-def _workspace(ws, dim, n, rows, heads, kv_heads, prefill, device):
-    need = workspace_bytes(dim, n, rows, heads, kv_heads, prefill)
+    need = workspace_bytes(dim, n, tokens, heads, ps[1], ps[2], max_pages, window, sinks, starts is not None)
     if ws is None:
-        return torch.empty(need, dtype=torch.uint8, device=device), need
-    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
         raise ValueError(f"ws must be a contiguous uint8 tensor of at least {need} bytes")
-    return ws, ws.numel()
+    p = _lib.ptr
+    rc = call(p(q), tag, *q_args, p(k_pages), p(v_pages), ks[0], ks[1], ks[2],
+              *((n, tokens // n if n else 0) if starts is None else (tokens, p(starts), n)), heads, ps[1], dim, ps[2], ps[0],
+              p(page_table), rows, max_pages, p(lengths), p(ids), window, sinks, scale, p(out), p(lse), p(ws), need, p(err),
+              _lib.stream())
+    if rc:
+        _lib.check(rc, what)
+    return out
 
 
 def attn_decode(q, k_pages, v_pages, page_table, lengths, out=None, *, lse=None, scale=None, window: int = 0,
@@ -88,19 +103,12 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, out=None, *, lse=None,
     """q [n, q_len, heads, head_dim] -> out of the same shape: the ``q_len`` newest tokens of every sequence (one of a
     decode step, a few of a speculative verify; q_len * heads / kv_heads <= 128). ``scale`` defaults to
     1 / sqrt(head_dim)."""
-    if q.dim() != 4 or q.stride(3) != 1:
+    qs = q.stride()
+    if len(qs) != 4 or qs[3] != 1:
         raise ValueError("q must be [n, q_len, heads, head_dim] with a contiguous head_dim")
     n, q_len, heads, dim = q.shape
-    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out,
-                               lse)
-    ws, ws_bytes = _workspace(ws, dim, n, n * q_len, heads, k_pages.shape[1], False, q.device)
-    p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
-    rc = _lib.lib().ssb_attn_decode(
-        p(q), tag, qs[0], qs[1], qs[2], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], n, q_len, heads, kp[1], dim, kp[2],
-        kp[0], p(page_table), rows, page_table.shape[1], p(lengths), p(ids), window, sinks,
-        1.0 / math.sqrt(dim) if scale is None else scale, p(out), p(lse), p(ws), ws_bytes, p(err), _lib.stream())
-    _lib.check(rc, "attn_decode")
-    return out
+    return _attend(_lib.lib().ssb_attn_decode, "attn_decode", q, heads, dim, n, n * q_len, None, qs[:3], k_pages, v_pages,
+                   page_table, lengths, out, lse, scale, window, sinks, ids, err, ws)
 
 
 def attn_prefill(q, k_pages, v_pages, page_table, lengths, starts, out=None, *, lse=None, scale=None, window: int = 0,
@@ -108,19 +116,11 @@ def attn_prefill(q, k_pages, v_pages, page_table, lengths, starts, out=None, *, 
     """q [rows, heads, head_dim] -> out of the same shape. Rows ``starts[b]`` to ``starts[b + 1]`` (int32 [n + 1], on the
     device, rising) are the newest tokens of sequence b: whole prompts, or chunks after cached ones. Rows outside
     every sequence are not written."""
-    if q.dim() != 3 or q.stride(2) != 1:
+    qs = q.stride()
+    if len(qs) != 3 or qs[2] != 1:
         raise ValueError("q must be [rows, heads, head_dim] with a contiguous head_dim")
     if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector of at least one element")
     total, heads, dim = q.shape
-    n = starts.numel() - 1
-    tag, ks, rows, out = _common(q, heads, dim, k_pages, v_pages, page_table, lengths, n, ids, window, sinks, scale, err, out,
-                               lse)
-    ws, ws_bytes = _workspace(ws, dim, n, total, heads, k_pages.shape[1], True, q.device)
-    p, qs, kp = _lib.ptr, q.stride(), k_pages.shape
-    rc = _lib.lib().ssb_attn_prefill(
-        p(q), tag, qs[0], qs[1], p(k_pages), p(v_pages), ks[0], ks[1], ks[2], total, p(starts), n, heads, kp[1], dim,
-        kp[2], kp[0], p(page_table), rows, page_table.shape[1], p(lengths), p(ids), window, sinks,
-        1.0 / math.sqrt(dim) if scale is None else scale, p(out), p(lse), p(ws), ws_bytes, p(err), _lib.stream())
-    _lib.check(rc, "attn_prefill")
-    return out
+    return _attend(_lib.lib().ssb_attn_prefill, "attn_prefill", q, heads, dim, starts.shape[0] - 1, total, starts, qs[:2],
+                   k_pages, v_pages, page_table, lengths, out, lse, scale, window, sinks, ids, err, ws)

@@ -182,9 +182,11 @@ def test_pages_behind_the_window_are_not_read():
 
 
 def test_results_repeat_and_a_batch_equals_itself_in_a_graph():
-    k, v, table, lens, g = _cache([700, 30, 2000], 2, 128, 16, BF)
+    k, v, table, lens, g = _cache([700, 30, 9000], 2, 128, 16, BF)
     q = _q(g, 3, 16, 2, 128, BF).unflatten(0, (3, 1))
-    ws = torch.empty(workspace_bytes(128, 3, 3, 16, 2), dtype=torch.uint8, device="cuda")
+    assert table.shape[1] * 16 > 8 * 8 * 128          # a table that calls for the split over blocks, with its workspace
+    ws = torch.empty(workspace_bytes(128, 3, 3, 16, 2, 16, table.shape[1]), dtype=torch.uint8, device="cuda")
+    assert ws.numel() > 0
     out, ref = torch.empty(q.shape, dtype=BF, device="cuda"), attn_decode(q, k, v, table, lens)
     graph = torch.cuda.CUDAGraph()
     attn_decode(q, k, v, table, lens, out, ws=ws)

@@ -120,13 +120,13 @@ def _decode_args(**change):
 
 
 @pytest.mark.parametrize("change,want", [
-    (dict(), _lib.SSB_EINVAL),                                     # no workspace
+    (dict(mp=1 << 16), _lib.SSB_EINVAL),                           # no workspace
     (dict(q_type=_lib.F32), _lib.SSB_EINVAL), (dict(dim=96), _lib.SSB_EUNSUPPORTED),
     (dict(q_len=65), _lib.SSB_EUNSUPPORTED), (dict(heads=5), _lib.SSB_EINVAL), (dict(kv=0), _lib.SSB_EINVAL),
     (dict(ps=0), _lib.SSB_EINVAL), (dict(pages=0), _lib.SSB_EINVAL), (dict(rows=0), _lib.SSB_EINVAL),
     (dict(mp=1 << 28), _lib.SSB_EINVAL), (dict(window=-1), _lib.SSB_EINVAL), (dict(sinks=-1), _lib.SSB_EINVAL),
     (dict(st=63), _lib.SSB_EINVAL), (dict(qh=4), _lib.SSB_EINVAL), (dict(k=72), _lib.SSB_EINVAL),
     (dict(scale=-1.0), _lib.SSB_EINVAL), (dict(n=-1), _lib.SSB_EINVAL), (dict(n=0), _lib.SSB_OK), (dict(q_len=0), _lib.SSB_OK),
-    (dict(q=None, ws_bytes=1 << 40), _lib.SSB_EINVAL), (dict(ws=None, ws_bytes=1 << 40), _lib.SSB_EINVAL)])
+    (dict(q=None, ws_bytes=1 << 40), _lib.SSB_EINVAL), (dict(ws=None, ws_bytes=1 << 40, mp=1 << 16), _lib.SSB_EINVAL)])
 def test_c_attention_refusals(change, want):
     assert _lib.lib().ssb_attn_decode(*_decode_args(**change)) == want
