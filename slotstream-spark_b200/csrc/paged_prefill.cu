@@ -37,10 +37,15 @@ namespace {
 
 template <int D>
 struct Cfg {
-  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = 64, SLOTS = D == 64 ? 16 : D == 128 ? 10 : 5;
-  static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
+  static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = 64;
+  // At head size 256 Q goes to TMEM: its 64 KB of shared memory are two more slots of the ring, whose depth bounds that
+  // size (with 5 slots instead of 7, 0.98 ms for 2 x 2,048 tokens after 14K and 3K; REPLACE256 ms now).
+  static constexpr bool Q_IN_TMEM = D == 256;
+  static constexpr int SLOTS = D == 64 ? 16 : D == 128 ? 10 : 7;
+  static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = Q_IN_TMEM ? 0 : MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
-  static constexpr int S_COL = NT * D;             // TMEM columns: the accumulators, then two buffers of S / P a row tile
+  // TMEM columns: the accumulators, Q (two elements a column), two buffers of S / P a row tile
+  static constexpr int Q_COL = NT * D, S_COL = Q_COL + (Q_IN_TMEM ? D / 2 : 0);
   static_assert(S_COL + NT * 2 * T <= 512, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 1;
@@ -54,8 +59,12 @@ struct __align__(16) Joint {
   int h, r0, rows, q0, slot, pieces, pad0, pad1;
 };
 
-// Tensor maps of a call: q [rows, heads, dim] in boxes of 128 flat rows x 64, k and v [pages, kv_heads, page, dim] in boxes of
-// page_rows tokens x 64.
+// Tiles of K and V lie in shared memory as groups of 8 tokens, in each of them 64 dims after 64 dims, as 8 rows of 128 swizzled
+// bytes: [T / 8][D / 64][8][128 B]. So the tokens of a page, with all their dims, are one run of it and come as one box
+// (with a box for every 64 dims, 2 KB each at pages of 16 tokens, head size 256 was bound by the number of boxes).
+//
+// Tensor maps of a call: q [rows, heads, dim] in boxes of 128 flat rows x 64; k and v as [page and head, page / 8, dim / 64, 8, 64]
+// in boxes of page_rows tokens x dim.
 struct Maps {
   CUtensorMap q, k, v;
 };
@@ -67,6 +76,7 @@ struct Work {
   Joint* joints;
   int max_units, max_slots;
   int page_rows, q_boxes;      // tokens of a K / V box, 0: by cp.async; whether Q comes in boxes
+  int page_heads;              // steps of the key head's stride from page to page
 };
 
 SSB_DEV int block_scan(int v, int* part, int* total) {
@@ -250,40 +260,40 @@ SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFF
 // the one thread that issues the products off the critical path -- with descriptors built from scratch it took about 100
 // cycles an instruction, more than the instruction itself.
 SSB_DEV uint32_t desc_lo(uint32_t smem_addr, uint32_t lead) { return (smem_addr >> 4) | (lead >> 4) << 16; }
-constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;     // 1024 bytes between groups of 8 rows, 128-byte swizzle
+constexpr uint32_t desc_hi(uint32_t group) { return (group >> 4) | 1u << 14 | 2u << 29; }   // bytes between groups of 8 rows
 // K-major tile (rows of 64 elements of the summed index); `lead` is not used by the swizzled form.
 constexpr uint32_t LEAD_K = 16;
 
-// One box of a 3-D / 4-D tensor map; the bytes are counted on `bar`.
+// One box of a 3-D / 5-D tensor map; the bytes are counted on `bar`.
 SSB_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-SSB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+SSB_DEV void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int v, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::
+          "r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
       : "memory");
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T.
-SSB_DEV void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+SSB_DEV void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                     uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n}\n" ::"r"(tmem_d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column. B's rows are the
-// summed index (tokens); its 128-byte panels hold 64 of the N index and lie the descriptor's lead apart.
-SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem]: the A rows are TMEM lanes, two 16-bit elements of a row per column.
+SSB_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 template <typename E>
@@ -413,7 +423,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     const int t = (warp - MMA) % NT;
     const bool scores = warp < MMA + NT;
     const uint32_t q_lo = desc_lo(smem_u32(sq) + t * 128 * 128, LEAD_K), k_lo = desc_lo(smem_u32(ring), LEAD_K),
-                   v_lo = desc_lo(smem_u32(ring), T * 128);
+                   v_lo = desc_lo(smem_u32(ring), 1024);
+    constexpr uint32_t GROUP = D / 64 * 1024, HI_Q = desc_hi(1024), HI_KV = desc_hi(GROUP);
     // A commit costs the tensor cores about 40 cycles. With a long ring its slots are given back by plain arrivals, when a
     // later wait shows that the product has ended; with a short one (size 256) that would be too late.
     constexpr bool FREE_BY_COMMIT = SLOTS < 8;
@@ -435,9 +446,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
           tc_fence_after();
           const uint32_t kd = k_lo + slot * (C::SLOT >> 4);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), kd + (((k / 4) * (T * 128) + (k % 4) * 32) >> 4),
-                    ID_S, k > 0);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t kk = kd + (((k / 4) * 1024 + (k % 4) * 32) >> 4);
+            if constexpr (C::Q_IN_TMEM) umma_ts(sd, tmem + C::Q_COL + k * 8, kk, HI_KV, ID_S, k > 0);
+            else umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), HI_Q, kk, HI_KV, ID_S, k > 0);
+          }
           umma_commit(s_full + buf);
           if (FREE_BY_COMMIT) umma_commit(empty + slot);
         } else {
@@ -449,7 +462,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
           tc_fence_after();
           const uint32_t vd = v_lo + slot * (C::SLOT >> 4), od = tmem + t * D;
 #pragma unroll
-          for (int k = 0; k < T / 16; ++k) umma_ts(od, sd + k * 8, vd + (k * 2048 >> 4), ID_O, i > u.i0 || k > 0);
+          for (int k = 0; k < T / 16; ++k) umma_ts(od, sd + k * 8, vd + (k * 2 * GROUP >> 4), HI_KV, ID_O, i > u.i0 || k > 0);
           umma_commit(o_done + buf);
           if (FREE_BY_COMMIT) umma_commit(empty + slot);
         }
@@ -488,13 +501,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
       const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
       const int32_t* trow = a.table + (int64_t)max(u.row, 0) * a.max_pages;
-      if (qn && !wait(q_empty, (qn - 1) & 1)) {
+      if (!C::Q_IN_TMEM && qn && !wait(q_empty, (qn - 1) & 1)) {
         ok = false;
         break;
       }
       ++qn;
-      const bool boxes = w.q_boxes != 0;
-      if (boxes) {
+      const bool boxes = C::Q_IN_TMEM || w.q_boxes != 0;      // nothing of Q among the copies
+      if constexpr (C::Q_IN_TMEM) {
+      } else if (boxes) {
         constexpr int N = NT * (D / 64);               // one box per row tile and 64 columns
         if (pt < N) {
           const int t = pt % NT, c = pt / NT;
@@ -539,16 +553,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
         }
         for (; first < upto; ++first) mbar_arrive(full + first % SLOTS);
       };
-      // A tile whose tokens are all seen by some query comes as boxes, one page's tokens x 64 columns each, box pt by
-      // thread pt; others, and pages that do not divide a tile, row by row, with zeros for what nobody sees.
-      constexpr int COLS = D / 64;
-      const int n_boxes = w.page_rows ? T / w.page_rows * COLS : 0;
+      // A tile whose tokens are all seen by some query comes as boxes, one page's tokens each, box pt by thread pt; others,
+      // and pages that do not divide a tile, row by row, with zeros for what nobody sees.
+      const int n_boxes = w.page_rows ? T / w.page_rows : 0;
       auto boxed = [&](int i) {
         const int t = tile_token(rg, i, T);
         return w.page_rows && t + T - 1 <= p_hi && (a.window == 0 || p_lo - t < a.window || t + T <= a.sinks);
       };
       auto box_page = [&](int i) {                    // page of this thread's box
-        return i < u.i1 && pt < n_boxes ? trow[page_of(a, tile_token(rg, i, T) + pt / COLS * w.page_rows)] : 0;
+        return i < u.i1 && pt < n_boxes ? trow[page_of(a, tile_token(rg, i, T) + pt * w.page_rows)] : 0;
       };
       bool as_box = boxed(u.i0);
       long long off = as_box ? -1 : offset_of(u.i0);
@@ -566,8 +579,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
               mbar_arrive(q_full);
             }
           }
-          const int t0 = tile_token(rg, i, T) + pt / COLS * w.page_rows, in_page = t0 - page_of(a, t0) * a.page_size;
-          const uint32_t at = (pt % COLS) * (T * 128) + pt / COLS * w.page_rows * 128;
+          const int t0 = tile_token(rg, i, T) + pt * w.page_rows, in_page = t0 - page_of(a, t0) * a.page_size;
+          const uint32_t at = pt * w.page_rows * (D * 2);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (ok && kv >= SLOTS && !wait(empty + kv % SLOTS, kv / SLOTS - 1)) ok = false;
@@ -576,13 +589,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
             if (pt >= n_boxes) {
               mbar_arrive(bar_full);
             } else if (page >= 0 && page < a.pages) {
-              mbar_expect_tx(bar_full, w.page_rows * 128);
-              tma_load_4d(smem_u32(ring + (kv % SLOTS) * C::SLOT) + at, x ? &maps.v : &maps.k, (pt % COLS) * 64, in_page, u.h, page,
-                          bar_full);
+              mbar_expect_tx(bar_full, w.page_rows * (D * 2));
+              tma_load_5d(smem_u32(ring + (kv % SLOTS) * C::SLOT) + at, x ? &maps.v : &maps.k, 0, 0, 0, in_page >> 3,
+                          page * w.page_heads + u.h, bar_full);
             } else {                                  // a missing page reads as zeros
               set_err(a.err, SSB_ERR_PAGE_RANGE);
               uint4* z = (uint4*)(ring + (kv % SLOTS) * C::SLOT + at);
-              for (int y = 0; y < w.page_rows * 8; ++y) z[y] = make_uint4(0, 0, 0, 0);
+              for (int y = 0; y < w.page_rows * (D / 8); ++y) z[y] = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
               mbar_arrive(bar_full);
             }
@@ -606,7 +619,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
               const int r = v * RPP + lane / CPR, c = lane % CPR;
               const long long o = __shfl_sync(0xFFFFFFFFu, off, r);
               const uint32_t row = pw * (T / 4) + r;
-              cp_async16(dst + (c >> 3) * (T * 128) + swz128(row, c & 7), base + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+              cp_async16(dst + (row >> 3) * (D * 16) + (c >> 3) * 1024 + swz128(row & 7, c & 7), base + (o < 0 ? 0 : o) + c * 8,
+                         o < 0 ? 0 : 16);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             ++kv;
@@ -629,13 +643,39 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     Unit u;
-    uint32_t tn = 0;
+    uint32_t tn = 0, qn = 0;
     bool ok = true;
     while (ok && next_unit(u)) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
       const int pos = p + min(f0 + row, last) / a.group;       // rows past the last: zero queries, never written
       const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
+      if constexpr (C::Q_IN_TMEM) {                   // this thread's row of Q, once the last unit's S are done
+        if (qn && !warp_wait(q_empty, qn - 1)) {
+          ok = false;
+          break;
+        }
+        ++qn;
+        tc_fence_after();
+        const int f = min(f0 + row, last), tk = f / a.group;
+        const uint16_t* src = a.q + (u.q0 + (int64_t)tk) * a.q_tok + (u.h * a.group + f - tk * a.group) * a.q_head;
+#pragma unroll 2
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[16];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint4 v = __ldg((const uint4*)(src + c * 32 + x * 8));
+            r[4 * x] = v.x;
+            r[4 * x + 1] = v.y;
+            r[4 * x + 2] = v.z;
+            r[4 * x + 3] = v.w;
+          }
+          tmem_st16(lane_base + C::Q_COL + c * 16, r);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(q_full);
+      }
       float m = -INFINITY, l = 0.f;
       for (int i = u.i0; i < u.i1; ++i, ++tn) {
         const uint32_t buf = 2 * t + (tn & 1), sc = lane_base + C::S_COL + buf * T;
@@ -822,7 +862,7 @@ EncodeFn encode_fn() {
 }
 bool encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
             const cuuint32_t* box) {
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i + 1 < rank; ++i)                 // what the encoder refuses goes by cp.async
     if (strides[i] == 0 || strides[i] >= (1ull << 40)) return false;
   EncodeFn f = encode_fn();
@@ -830,18 +870,22 @@ bool encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint6
                 strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// Boxes need pages that divide a tile or are divided by it, at least 8 tokens long (shorter ones would be many small
-// boxes), and a group that divides the 128 rows of a row tile.
+// Boxes need pages that divide a tile or are divided by it, in groups of 8 tokens, page strides that are whole numbers of
+// head strides (page and head are one index of the map), and a group that divides the 128 rows of a row tile.
 void make_maps(Maps& m, Work& w, const Args& a, bool bf16, int dim, int tile) {
-  w.page_rows = w.q_boxes = 0;
-  if (a.page_size >= 8 && (a.page_size & (a.page_size - 1)) == 0) {
+  w.page_rows = w.q_boxes = w.page_heads = 0;
+  if (a.page_size >= 8 && (a.page_size & (a.page_size - 1)) == 0 && a.st > 0 && a.sh > 0 && a.sp > 0 && a.sp % a.sh == 0 &&
+      ((int64_t)a.pages * (a.sp / a.sh) + a.kv_heads) < 0x7FFFFFFF) {
     const int rows = a.page_size < tile ? a.page_size : tile;
-    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)a.page_size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)a.st * 2, (cuuint64_t)a.sh * 2, (cuuint64_t)a.sp * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
-    if (a.st > 0 && a.sh > 0 && a.sp > 0 && encode(&m.k, bf16, 4, a.k, dims, strides, box) &&
-        encode(&m.v, bf16, 4, a.v, dims, strides, box))
+    const cuuint64_t steps = (cuuint64_t)(a.sp / a.sh);
+    const cuuint64_t dims[5] = {64, 8, (cuuint64_t)dim / 64, (cuuint64_t)a.page_size / 8,
+                                (cuuint64_t)(a.pages - 1) * steps + (cuuint64_t)a.kv_heads};
+    const cuuint64_t strides[4] = {(cuuint64_t)a.st * 2, 128, (cuuint64_t)a.st * 16, (cuuint64_t)a.sh * 2};
+    const cuuint32_t box[5] = {64, 8, (cuuint32_t)dim / 64, (cuuint32_t)rows / 8, 1};
+    if (encode(&m.k, bf16, 5, a.k, dims, strides, box) && encode(&m.v, bf16, 5, a.v, dims, strides, box)) {
       w.page_rows = rows;
+      w.page_heads = (int)steps;
+    }
   }
   if (128 % a.group == 0) {
     const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.heads, (cuuint64_t)a.rows};
