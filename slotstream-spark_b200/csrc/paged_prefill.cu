@@ -38,14 +38,10 @@ namespace {
 template <int D>
 struct Cfg {
   static constexpr int NT = D == 256 ? 1 : 2, MB = 128 * NT, T = 64;
-  // At head size 256 Q goes to TMEM: its 64 KB of shared memory are two more slots of the ring, whose depth bounds that
-  // size (with 5 slots instead of 7, 0.98 ms for 2 x 2,048 tokens after 14K and 3K; REPLACE256 ms now).
-  static constexpr bool Q_IN_TMEM = D == 256;
-  static constexpr int SLOTS = D == 64 ? 16 : D == 128 ? 10 : 7;
-  static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = Q_IN_TMEM ? 0 : MB * D * 2, CTL = 512;
+  static constexpr int SLOTS = D == 64 ? 16 : D == 128 ? 10 : 5;
+  static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
-  // TMEM columns: the accumulators, Q (two elements a column), two buffers of S / P a row tile
-  static constexpr int Q_COL = NT * D, S_COL = Q_COL + (Q_IN_TMEM ? D / 2 : 0);
+  static constexpr int S_COL = NT * D;             // TMEM columns: the accumulators, then two buffers of S / P a row tile
   static_assert(S_COL + NT * 2 * T <= 512, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 1;
@@ -448,8 +444,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t kk = kd + (((k / 4) * 1024 + (k % 4) * 32) >> 4);
-            if constexpr (C::Q_IN_TMEM) umma_ts(sd, tmem + C::Q_COL + k * 8, kk, HI_KV, ID_S, k > 0);
-            else umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), HI_Q, kk, HI_KV, ID_S, k > 0);
+            umma_ss(sd, q_lo + (((k / 4) * (C::MB * 128) + (k % 4) * 32) >> 4), HI_Q, kk, HI_KV, ID_S, k > 0);
           }
           umma_commit(s_full + buf);
           if (FREE_BY_COMMIT) umma_commit(empty + slot);
@@ -501,14 +496,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
       const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
       const int32_t* trow = a.table + (int64_t)max(u.row, 0) * a.max_pages;
-      if (!C::Q_IN_TMEM && qn && !wait(q_empty, (qn - 1) & 1)) {
+      if (qn && !wait(q_empty, (qn - 1) & 1)) {
         ok = false;
         break;
       }
       ++qn;
-      const bool boxes = C::Q_IN_TMEM || w.q_boxes != 0;      // nothing of Q among the copies
-      if constexpr (C::Q_IN_TMEM) {
-      } else if (boxes) {
+      const bool boxes = w.q_boxes != 0;
+      if (boxes) {
         constexpr int N = NT * (D / 64);               // one box per row tile and 64 columns
         if (pt < N) {
           const int t = pt % NT, c = pt / NT;
@@ -567,6 +561,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       long long off = as_box ? -1 : offset_of(u.i0);
       int page = as_box ? box_page(u.i0) : 0;
       for (int i = u.i0; i < u.i1 && ok; ++i) {
+        asm volatile("" : "+r"(page), "+l"(off));     // loaded a tile ago; their checks stay behind this point
         const bool box_next = i + 1 < u.i1 && boxed(i + 1);
         const long long off_next = box_next ? -1 : offset_of(i + 1);
         const int page_next = box_next ? box_page(i + 1) : 0;
@@ -643,39 +638,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     Unit u;
-    uint32_t tn = 0, qn = 0;
+    uint32_t tn = 0;
     bool ok = true;
     while (ok && next_unit(u)) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
       const int pos = p + min(f0 + row, last) / a.group;       // rows past the last: zero queries, never written
       const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
-      if constexpr (C::Q_IN_TMEM) {                   // this thread's row of Q, once the last unit's S are done
-        if (qn && !warp_wait(q_empty, qn - 1)) {
-          ok = false;
-          break;
-        }
-        ++qn;
-        tc_fence_after();
-        const int f = min(f0 + row, last), tk = f / a.group;
-        const uint16_t* src = a.q + (u.q0 + (int64_t)tk) * a.q_tok + (u.h * a.group + f - tk * a.group) * a.q_head;
-#pragma unroll 2
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[16];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint4 v = __ldg((const uint4*)(src + c * 32 + x * 8));
-            r[4 * x] = v.x;
-            r[4 * x + 1] = v.y;
-            r[4 * x + 2] = v.z;
-            r[4 * x + 3] = v.w;
-          }
-          tmem_st16(lane_base + C::Q_COL + c * 16, r);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(q_full);
-      }
       float m = -INFINITY, l = 0.f;
       for (int i = u.i0; i < u.i1; ++i, ++tn) {
         const uint32_t buf = 2 * t + (tn & 1), sc = lane_base + C::S_COL + buf * T;
