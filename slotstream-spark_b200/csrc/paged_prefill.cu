@@ -41,8 +41,9 @@ struct Cfg {
   static constexpr int SLOTS = D == 64 ? 16 : D == 128 ? 10 : 5;
   static constexpr int CPR = D / 8, SLOT = T * D * 2, QB = MB * D * 2, CTL = 512;
   static constexpr int SMEM = QB + SLOTS * SLOT + CTL, THREADS = (NT + 2) * 128;
-  static constexpr int S_COL = NT * D;             // TMEM columns: the accumulators, then two buffers of S / P a row tile
-  static_assert(S_COL + NT * 2 * T <= 512, "TMEM");
+  // TMEM columns: the accumulators, then as many buffers of S / P a row tile as fit
+  static constexpr int S_COL = NT * D, NBUF = (512 - S_COL) / (NT * T);
+  static_assert(NBUF >= 2 && NT * NBUF <= 6, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 1;
 
@@ -346,13 +347,13 @@ SSB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: 
 template <typename E, int D>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_constant__ Maps maps, Args a, Work w) {
   using C = Cfg<D>;
-  constexpr int NT = C::NT, T = C::T, CPR = C::CPR, SLOTS = C::SLOTS;
+  constexpr int NT = C::NT, T = C::T, CPR = C::CPR, SLOTS = C::SLOTS, NBUF = C::NBUF;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
   uint8_t* ring = smem + C::QB;
   uint64_t* bar = (uint64_t*)(ring + SLOTS * C::SLOT);
   uint64_t *q_full = bar, *q_empty = bar + 1, *u_full = bar + 2, *u_empty = bar + 4, *drained = bar + 6,
-           *s_full = bar + 10, *p_full = bar + 14, *o_done = bar + 18, *full = bar + 22, *empty = full + SLOTS;
+           *s_full = bar + 10, *p_full = bar + 16, *o_done = bar + 22, *full = bar + 28, *empty = full + SLOTS;
   int* u_slot = (int*)(empty + SLOTS);             // unit numbers handed out, two in flight
   uint32_t* tmem_slot = (uint32_t*)(u_slot + 2);
   int* failed = (int*)(tmem_slot + 1);
@@ -371,8 +372,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       mbar_init(u_full + i, 1);
       mbar_init(u_empty + i, NT * 128 + 128 + 2 * NT);
     }
-    for (int i = 0; i < 4; ++i) {                    // s_full, p_full, o_done: [row tile][buffer]
-      mbar_init(drained + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(drained + i, 1);
+    for (int i = 0; i < NT * NBUF; ++i) {            // [row tile][buffer]
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
       mbar_init(o_done + i, 1);
@@ -432,13 +433,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       if (scores) need(q_full, qn++);
 #pragma unroll 1
       for (int i = u.i0; i < u.i1 && ok; ++i, ++tn, kv += 2) {
-        const uint32_t buf = 2 * t + (tn & 1), use = tn >> 1, sd = tmem + C::S_COL + buf * T;
+        const uint32_t buf = NBUF * t + tn % NBUF, use = tn / NBUF, sd = tmem + C::S_COL + buf * T;
         if (scores) {
           const uint32_t slot = kv % SLOTS;
           need(full + slot, kv / SLOTS);
           if (use) need(o_done + buf, use - 1);     // the product that read P from this buffer
           if (!ok) break;
-          if (!FREE_BY_COMMIT && tn >= 2) mbar_arrive(empty + (kv - 3) % SLOTS);      // and the values of two tiles before
+          if (!FREE_BY_COMMIT && use) mbar_arrive(empty + (kv + 1 - 2 * NBUF) % SLOTS);      // and its values
           tc_fence_after();
           const uint32_t kd = k_lo + slot * (C::SLOT >> 4);
 #pragma unroll
@@ -647,8 +648,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
       float m = -INFINITY, l = 0.f;
       for (int i = u.i0; i < u.i1; ++i, ++tn) {
-        const uint32_t buf = 2 * t + (tn & 1), sc = lane_base + C::S_COL + buf * T;
-        if (!warp_wait(s_full + buf, tn >> 1)) {
+        const uint32_t buf = NBUF * t + tn % NBUF, sc = lane_base + C::S_COL + buf * T;
+        if (!warp_wait(s_full + buf, tn / NBUF)) {
           ok = false;
           break;
         }
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
         } else {
           const bool raise = mx > m + 8.f;
           if (__any_sync(0xFFFFFFFFu, raise)) {
-            if (!warp_wait(o_done + (buf ^ 1), (tn - 1) >> 1)) {     // the product of the tile before adds to the sum
+            if (!warp_wait(o_done + NBUF * t + (tn - 1) % NBUF, (tn - 1) / NBUF)) {     // the product of the tile before adds to the sum
               ok = false;
               break;
             }
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
         tc_fence_before();
         mbar_arrive(p_full + buf);
       }
-      if (!ok || !warp_wait(o_done + 2 * t + ((tn - 1) & 1), (tn - 1) >> 1)) {
+      if (!ok || !warp_wait(o_done + NBUF * t + (tn - 1) % NBUF, (tn - 1) / NBUF)) {
         ok = false;
         break;
       }
