@@ -25,21 +25,21 @@ struct Cache {
   int32_t *table, *err, *scratch;
 };
 
-// scratch: [0] copies, [1] rows to share, [2] live pages of a compaction; then src / dst of the copies, then two
-// arrays of `pages` (page lists) and two of `seqs` (per-sequence counts).
+// scratch: [0] copies, [1] rows to share, [2] live pages of a compaction; then src / dst of the copies, a page list, two
+// arrays of `seqs` (per-sequence counts), and one of pages + 2 seqs (counts of 32 table entries each).
 struct Scratch {
-  int32_t *head, *src, *dst, *list, *list2, *num, *num2;
+  int32_t *head, *src, *dst, *list, *num, *num2, *part;
 };
-__host__ __device__ inline int64_t scratch_ints(int64_t pages, int64_t seqs) { return 8 + 4 * pages + 2 * seqs; }
+__host__ __device__ inline int64_t scratch_ints(int64_t pages, int64_t seqs) { return 8 + 4 * pages + 4 * seqs; }
 SSB_DEV Scratch scratch_of(const Cache& c) {
   Scratch s;
   s.head = c.scratch;
   s.src = s.head + 8;
   s.dst = s.src + c.pages;
   s.list = s.dst + c.pages;
-  s.list2 = s.list + c.pages;
-  s.num = s.list2 + c.pages;
+  s.num = s.list + c.pages;
   s.num2 = s.num + c.seqs;
+  s.part = s.num2 + c.seqs;
   return s;
 }
 
@@ -113,6 +113,8 @@ SSB_DEV bool seen_before(uint32_t* bitmap, int s) {
   return atomicOr(&bitmap[s >> 5], bit) & bit;
 }
 
+// Allocation: the table entries that the new tokens fall into, in runs of 32 (a warp each), are counted where they lack a
+// page, the counts are scanned, and the lowest free pages dealt out in that order.
 __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __restrict__ ids,
                                                    const int32_t* __restrict__ counts, int n) {
   extern __shared__ uint32_t bitmap[];
@@ -123,72 +125,92 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
   for (int i = threadIdx.x; i < (c.seqs + 31) >> 5; i += PLAN_T) bitmap[i] = 0;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
-  for (int i = warp; i < n; i += PLAN_T / 32) {
-    const int s = ids[i], add = counts[i];
-    int wrong = 0, need = 0;
-    if (s < 0 || s >= c.seqs || add < 0) {
-      wrong = SSB_ERR_SEQUENCE;
-    } else {
-      int dup = 0;
-      if (lane == 0) dup = seen_before(bitmap, s);
-      if (__shfl_sync(0xFFFFFFFFu, dup, 0)) wrong = SSB_ERR_SEQUENCE;
-      const int64_t len = c.lengths[s], now = len + add;
-      if (len < 0) {
-        wrong |= SSB_ERR_SEQUENCE;
-      } else if (now > (int64_t)c.max_pages * c.page_size) {
-        wrong |= SSB_ERR_NO_PAGES;
-      } else if (add > 0) {
-        const int j1 = (int)((now + c.page_size - 1) / c.page_size);
-        for (int j = (int)(len / c.page_size) + lane; j < j1; j += 32) {
-          const int p = c.table[(int64_t)s * c.max_pages + j];
-          if (p < 0) ++need;
-          else if (p >= c.pages) wrong |= SSB_ERR_PAGE_RANGE;
-          else if (c.refs[p] > 1) wrong |= SSB_ERR_SHARED_PAGE;
-        }
+  // entries of each sequence, its first run, and where in the table they begin; in shared memory where the call is small
+  __shared__ int s_num[PLAN_T], s_run[PLAN_T];
+  __shared__ int64_t s_at[PLAN_T];
+  int32_t *num = n <= PLAN_T ? s_num : sc.num, *run = n <= PLAN_T ? s_run : sc.num2;
+  int runs = 0;
+  // Every entry is a page of its own at the end, so more entries than pages cannot be had; then runs > pages / 32 + n.
+  const int most = c.pages / 32 + n;
+  for (int i0 = 0; i0 < n && runs <= most; i0 += PLAN_T) {
+    const int i = i0 + threadIdx.x;
+    int wrong = 0, e = 0;
+    if (i < n) {
+      const int s = ids[i], add = counts[i];
+      if (s < 0 || s >= c.seqs || add < 0 || seen_before(bitmap, s)) {
+        wrong = SSB_ERR_SEQUENCE;
+      } else {
+        const int64_t len = c.lengths[s], now = len + add;
+        if (len < 0) wrong = SSB_ERR_SEQUENCE;
+        else if (now > (int64_t)c.max_pages * c.page_size) wrong = SSB_ERR_NO_PAGES;
+        else if (add > 0) e = (int)((now + c.page_size - 1) / c.page_size - len / c.page_size);
+        if (n <= PLAN_T) s_at[i] = (int64_t)s * c.max_pages + len / c.page_size;
       }
-    }
-    need = __reduce_add_sync(0xFFFFFFFFu, need);
-    wrong = __reduce_or_sync(0xFFFFFFFFu, wrong);
-    if (lane == 0) {
-      sc.num[i] = need;
       if (wrong) atomicOr(&bad, wrong);
+      e = min(e, c.pages + 32);
     }
+    int total;
+    const int ex = block_scan((e + 31) >> 5, part, &total);
+    if (i < n) {
+      num[i] = e;
+      run[i] = runs + ex;
+    }
+    runs += total;
+  }
+  if (runs > most && threadIdx.x == 0) atomicOr(&bad, SSB_ERR_NO_PAGES);
+  __syncthreads();
+  if (bad) {
+    if (threadIdx.x == 0) set_err(c.err, bad);
+    return;
+  }
+  // run r: its sequence's table entry for this lane (nullptr past the last)
+  auto entry_of = [&](int r) -> int32_t* {
+    int lo = 0, hi = n;                                // the last i with run[i] <= r
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (run[mid] <= r) lo = mid;
+      else hi = mid;
+    }
+    const int k = (r - run[lo]) * 32 + lane;
+    if (k >= num[lo]) return nullptr;
+    if (n <= PLAN_T) return c.table + s_at[lo] + k;
+    const int s = ids[lo];
+    return c.table + (int64_t)s * c.max_pages + c.lengths[s] / c.page_size + k;
+  };
+  for (int r = warp; r < runs; r += PLAN_T / 32) {
+    const int32_t* e = entry_of(r);
+    const int p = e ? *e : 0;
+    const int wrong = !e || p < 0 ? 0 : p >= c.pages ? SSB_ERR_PAGE_RANGE : c.refs[p] > 1 ? SSB_ERR_SHARED_PAGE : 0;
+    const uint32_t lacks = __ballot_sync(0xFFFFFFFFu, e && p < 0);
+    if (wrong) atomicOr(&bad, wrong);
+    if (lane == 0) sc.part[r] = __popc(lacks);
   }
   __syncthreads();
-  int base = 0;
-  for (int i0 = 0; i0 < n; i0 += PLAN_T) {
-    const int i = i0 + threadIdx.x;
+  int need = 0;
+  for (int r0 = 0; r0 < runs; r0 += PLAN_T) {
+    const int r = r0 + threadIdx.x;
     int total;
-    const int ex = block_scan(i < n ? min(sc.num[i], c.pages + 1) : 0, part, &total);
-    if (i < n) sc.num2[i] = base + ex;
-    base = min(base + total, c.pages + 1);      // more than every page: refused below, no overflow
+    const int ex = block_scan(r < runs ? sc.part[r] : 0, part, &total);
+    if (r < runs) sc.part[r] = need + ex;
+    need += total;
   }
   __syncthreads();
   if (bad) {
     if (threadIdx.x == 0) set_err(c.err, bad);
     return;
   }
-  if (!take_pages(c, base, sc.list, part)) {
+  if (!take_pages(c, need, sc.list, part)) {
     if (threadIdx.x == 0) set_err(c.err, SSB_ERR_NO_PAGES);
     return;
   }
-  for (int i = warp; i < n; i += PLAN_T / 32) {
-    const int s = ids[i], add = counts[i];
-    const int64_t len = c.lengths[s], now = len + add;
-    const int j1 = (int)((now + c.page_size - 1) / c.page_size);
-    int at = sc.num2[i];
-    if (add > 0)
-      for (int j0 = (int)(len / c.page_size); j0 < j1; j0 += 32) {
-        const int j = j0 + lane;
-        int32_t* e = c.table + (int64_t)s * c.max_pages + j;
-        const bool lacks = j < j1 && *e < 0;
-        const uint32_t m = __ballot_sync(0xFFFFFFFFu, lacks);
-        if (lacks) *e = sc.list[at + __popc(m & lanemask_lt())];
-        at += __popc(m);
-      }
-    __syncwarp();
-    if (lane == 0) c.lengths[s] = (int32_t)now;
+  for (int r = warp; r < runs; r += PLAN_T / 32) {
+    int32_t* e = entry_of(r);
+    const bool lacks = e && *e < 0;
+    const uint32_t m = __ballot_sync(0xFFFFFFFFu, lacks);
+    if (lacks) *e = sc.list[sc.part[r] + __popc(m & lanemask_lt())];
   }
+  __syncthreads();                                     // entries are found through the old lengths
+  for (int i = threadIdx.x; i < n; i += PLAN_T) c.lengths[ids[i]] += counts[i];
 }
 
 __global__ void __launch_bounds__(PLAN_T) k_fork_plan(Cache c, const int32_t* __restrict__ parents,

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a, in
     *sum = all;
     return before + inc;
   };
-  if (!DIRECT && tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (!DIRECT && !a.desc_by_item && tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
   long long w0 = weight_of(tid), total;
   const long long inc0 = scan_block(w0, &total);
   const long long first_total = total;
@@ -463,8 +463,9 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a, in
     }
     if (tid == 0) {
       if (s.row < 0) set_err(a.err, SSB_ERR_SEQUENCE);
-      if (!DIRECT && i0 == 0 && !whole_item)
-        a.desc[blockIdx.x] = make_int4(b, item, (int)((item0 + rg.tiles - 1) / chunk), rows);
+      if (!DIRECT && i0 == 0 && (!whole_item || a.desc_by_item))
+        a.desc[a.desc_by_item ? b * a.kv_heads * nb + item : blockIdx.x] =
+            make_int4(whole_item ? -1 : b, item, blockIdx.x | rows << 24, (int)((item0 + rg.tiles - 1) / chunk));
     }
     if (DIRECT) return;
     __syncthreads();
@@ -472,33 +473,33 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a, in
   }
 }
 
-// Joins the pieces of the items that cross blocks: grid (blocks of the first kernel, RB), one row per block; desc[c] =
-// (sequence, item, last block, rows) when block c holds an item's first piece. Its pieces are slot 2c + 1 and the even
-// slots of the blocks after c, summed in that order.
-constexpr int JOIN_T = 256;
-template <typename E, int D, int ROWS>
-__global__ void __launch_bounds__(JOIN_T) k_attn_join(Args a) {
+// Joins the pieces of the items that cross blocks: grid (descriptors, RB), one row per block. Descriptors are one an item
+// where those are fewer, else one a block (of the item whose first piece it holds): (sequence or -1, item, first block and
+// rows, last block). The pieces are slot 2c + 1 of the first block and the even slots of the blocks after it, summed in that
+// order. JT threads: 1024 where items have many pieces.
+template <typename E, int D, int ROWS, int JT>
+__global__ void __launch_bounds__(JT) k_attn_join(Args a) {
   pdl_wait();
   const int4 d = a.desc[blockIdx.x];
-  const int r = blockIdx.y;
-  if (d.x < 0 || r >= d.w) return;
-  constexpr int LANES = D / 4, G = JOIN_T / LANES;    // threads of a row, groups that share the pieces
+  const int r = blockIdx.y, c0 = d.z & 0xFFFFFF;
+  if (d.x < 0 || r >= d.z >> 24) return;
+  constexpr int LANES = D / 4, G = JT / LANES;        // threads of a row, groups that share the pieces
   __shared__ float4 part[G][LANES];
-  __shared__ float factor[JOIN_T], warp_m[JOIN_T / 32], warp_l[JOIN_T / 32];
+  __shared__ float factor[JT], warp_m[JT / 32], warp_l[JT / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int c0 = blockIdx.x, n = d.z - c0 + 1, c = tid % LANES, g = tid / LANES;
+  const int n = d.w - c0 + 1, c = tid % LANES, g = tid / LANES;
   auto slot = [&](int i) { return (i == 0 ? 2 * (int64_t)c0 + 1 : 2 * (int64_t)(c0 + i)) * ROWS + r; };
   float m = -INFINITY;
-  for (int i = tid; i < n; i += JOIN_T) m = fmaxf(m, a.ml[slot(i)].x);
+  for (int i = tid; i < n; i += JT) m = fmaxf(m, a.ml[slot(i)].x);
   m = warp_max(m);
   if (lane == 0) warp_m[warp] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < JOIN_T / 32; ++w) m = fmaxf(m, warp_m[w]);
+  for (int w = 0; w < JT / 32; ++w) m = fmaxf(m, warp_m[w]);
   const float u = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += JOIN_T) {
+  for (int i0 = 0; i0 < n; i0 += JT) {
     __syncthreads();
     if (i0 + tid < n) {
       const float2 e = a.ml[slot(i0 + tid)];
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(JOIN_T) k_attn_join(Args a) {
       l += e.y * factor[tid];
     }
     __syncthreads();
-    const int k = min(n - i0, JOIN_T);
+    const int k = min(n - i0, JT);
 #pragma unroll 8
     for (int i = g; i < k; i += G) {
       const float f = factor[i];
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(JOIN_T) k_attn_join(Args a) {
   if (g) return;
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < JOIN_T / 32; ++w) l += warp_l[w];
+  for (int w = 0; w < JT / 32; ++w) l += warp_l[w];
 #pragma unroll
   for (int x = 1; x < G; ++x) {
     const float4 y = part[x][c];
@@ -630,13 +631,16 @@ int launch_rows(Args& a, uint8_t* ws, cudaStream_t stream) {
   a.desc = (int4*)(ws + l.desc);
   a.ml = (float2*)(ws + l.ml);
   a.acc = (float*)(ws + l.acc);
+  a.desc_by_item = items <= blocks;                   // the split is for decode calls only: the same items a sequence
   auto kern = k_attn_rows<E, D, RB, false>;
   static std::atomic<uint64_t> done{0};
   int rc = ssb_setup_kernel(done, "attn_decode", kern, SMEM<D, RB>);
   if (rc) return rc;
   rc = ssb_launch(kern, dim3(blocks), dim3(NW * 32), SMEM<D, RB>, stream, false, a, 1);
   if (rc) return rc;
-  return ssb_launch(k_attn_join<E, D, RB>, dim3(blocks, RB), dim3(JOIN_T), 0, stream, true, a);
+  const dim3 grid((unsigned)(a.desc_by_item ? items : blocks), RB);
+  if (items * 8 <= blocks) return ssb_launch(k_attn_join<E, D, RB, 1024>, grid, dim3(1024), 0, stream, true, a);
+  return ssb_launch(k_attn_join<E, D, RB, 256>, grid, dim3(256), 0, stream, true, a);
 }
 
 template <typename E>

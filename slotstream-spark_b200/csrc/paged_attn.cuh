@@ -29,7 +29,8 @@ struct Args {
   uint16_t* out;
   float* lse;
   int32_t* err;
-  int4* desc;                         // [blocks] items to join (see k_attn_join)
+  int4* desc;                         // items to join (see k_attn_join)
+  int desc_by_item;
   float2* ml;                         // [2 * blocks, RB] (max, sum) of the pieces, log2 domain
   float* acc;                         // [2 * blocks, RB, D]
 };
