@@ -489,13 +489,14 @@ int ssb_kv_compact(const ssb_kv_cache* c, void* stream);
  * softmax statistics and sums; the softmax weights are rounded to the inputs' type for the tensor cores), zero where
  * none is visible; lse (fp32, nullable) = log sum exp(scale * q . k), -inf there. q_type SSB_BF16 or SSB_F16, the cache
  * and out have the same. k / v: the layer's first key and value element in the pool, with page, head and token strides
- * in elements (multiples of 8; 16-byte aligned); pages, page_size (any), table [.., max_pages], lengths as above; ids
- * (nullable) maps batch row b to its table row, one of table_rows (others read as empty and set
- * SSB_ERR_SEQUENCE). What no query of the call sees is not read; a visible token whose
- * table entry lies outside [0, pages) reads as zeros and sets SSB_ERR_PAGE_RANGE. heads is a multiple of kv_heads,
- * query head h reads key head h / (heads / kv_heads); dim 64, 128 or 256; scale positive and finite. ws: workspace of ssb_attn_workspace bytes for
- * the call's sizes (rows = all query tokens; 0: ws may be NULL), contents irrelevant between calls; calls sharing it must
- * not overlap.
+ * in elements (multiples of 8; 16-byte aligned); pages, page_size (any), table [table_rows, max_pages], lengths
+ * [table_rows] as above; ids (nullable) maps batch row b to its table row (one out of range reads as empty and sets
+ * SSB_ERR_SEQUENCE). What no query of the call sees is not read: its value may be anything. A NaN or infinity in the
+ * value of a token that some queries of a sequence see spreads, as 0 x NaN, to others of the same tile. A visible token
+ * whose table entry lies outside [0, pages) reads as zeros and sets SSB_ERR_PAGE_RANGE. heads is a multiple of kv_heads,
+ * query head h reads key head h / (heads / kv_heads); dim 64, 128 or 256; scale positive and finite. ws: workspace of
+ * ssb_attn_workspace bytes for the call's sizes (rows = all query tokens; 0: ws may be NULL), contents irrelevant between
+ * calls; calls sharing it must not overlap.
  *
  * ssb_attn_decode: q [n, q_len, heads, dim] (strides in elements, multiples of 8), the q_len newest tokens of each
  * sequence (positions lengths - q_len ..; a position below 0 has no visible token). q_len * heads / kv_heads <= 128.

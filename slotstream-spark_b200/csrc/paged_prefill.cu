@@ -5,8 +5,8 @@
 // S = Q K^T from shared memory, and O += P V with P read from TMEM, where the softmax has put it.
 // What bounds it: the two products are 4 T MB D operations and the softmax T MB exponentials per tile; at head size
 // 128 the tensor cores and the 16 exponentials per clock of an SM need the same time, so both have to run all the time.
-// Hence two row tiles of 128 (NT = 2; one at head size 256, whose accumulator fills half of TMEM) and two buffers of S for
-// each: the S of the next tile is computed under the softmax of this one, so neither waits for the latency of the other
+// Hence two row tiles of 128 (NT = 2; one at head size 256, whose accumulator fills half of TMEM) and two to four buffers
+// of S for each: the S of the next tile is computed under the softmax of this one, so neither waits for the latency of the other
 // (about 350 cycles from an instruction's issue to a waiting thread).
 //
 // The running maximum is only raised when a row's maximum grows by more than 2^8 (log2 domain): p stays below 2^8, which
@@ -21,7 +21,8 @@
 // Tiles of 64 tokens: two buffers of S for two row tiles of head size 128 fill TMEM. Instructions of 64 columns cost 48
 // cycles for 32 columns' worth of work (operands read from shared memory), so the products of a pair of tiles take 2570
 // cycles per 128 tokens instead of 2050; single-buffered tiles of 128, where each S waits for the product before it, took
-// 4600 (32K tokens, window 4096: 2.16 ms against 1.96).
+// 4600 (32K tokens, 32 heads, 8 key heads, window 4096: 2.16 ms against 1.91, 1.08 PFLOP/s). At size 256 two chunks of 2,048
+// tokens after 14K and 3K take 0.61 ms (1.05 PFLOP/s), bound by the shared memory's bandwidth: 192 KB a tile and row tile.
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
@@ -412,8 +413,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     return range_of(a, p + u.r0 / a.group, p + (u.r0 + u.rows - 1) / a.group, T);
   };
 
-  if (warp >= MMA) {
-   if (warp < MMA + 2 * NT && lane == 0) {
+  if (warp >= MMA + 2 * NT || (warp >= MMA && lane > 0)) {
+    // the rest of the issuing warps
+  } else if (warp >= MMA) {
     // One warp per row tile and product: a thread that waits on a barrier between two products leaves the tensor cores
     // idle for about 170 cycles (its queue is short), unless another thread's products fill the gap.
     constexpr uint32_t ID_S = idesc_of<E>(128, T, false), ID_O = idesc_of<E>(128, D, true);
@@ -468,7 +470,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     if (!ok) give_up();
     umma_commit(drained + (warp - MMA));            // nothing of this thread's may run when TMEM goes
     if (!wait(drained + (warp - MMA), 0)) give_up();
-   }
   } else if (warp >= PROD) {
     const int pt = tid - PROD * 32, pw = pt >> 5;
     Unit u;
@@ -634,6 +635,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       if (ok) hand_over(kv);
     }
     cp_async_wait_all();
+    // No copy of this block's may be on its way when it ends (after a wait that gave up, one could be).
+    if (qn) ok = wait(q_full, qn - 1) && ok;
+    for (uint32_t n = kv > SLOTS ? kv - SLOTS : 0; n < kv; ++n) ok = wait(full + n % SLOTS, n / SLOTS) && ok;
     if (!ok) give_up();
   } else {
     const int t = warp >> 2, row = tid & 127;
@@ -679,7 +683,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
         } else {
           const bool raise = mx > m + 8.f;
           if (__any_sync(0xFFFFFFFFu, raise)) {
-            if (!warp_wait(o_done + NBUF * t + (tn - 1) % NBUF, (tn - 1) / NBUF)) {     // the product of the tile before adds to the sum
+            // the product of the tile before adds to the sum
+            if (!warp_wait(o_done + NBUF * t + (tn - 1) % NBUF, (tn - 1) / NBUF)) {
               ok = false;
               break;
             }
@@ -734,15 +739,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float v[32];
+        __syncwarp();                                  // the rows past the last skip the stores
         tmem_ld_row<32>(lane_base + t * D + c, v);
-        if (!in) continue;
-        if (u.slot < 0) {
+        if (in && u.slot < 0) {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             *(uint4*)(a.out + orow * D + c + 8 * x) =
                 make_uint4(pack2<E>(v[8 * x] * inv, v[8 * x + 1] * inv), pack2<E>(v[8 * x + 2] * inv, v[8 * x + 3] * inv),
                            pack2<E>(v[8 * x + 4] * inv, v[8 * x + 5] * inv), pack2<E>(v[8 * x + 6] * inv, v[8 * x + 7] * inv));
-        } else {
+        } else if (in) {
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             *(float4*)(a.acc + prow * D + c + 4 * x) = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
