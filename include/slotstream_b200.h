@@ -460,14 +460,19 @@ int ssb_kv_scratch_ints(int32_t pages, int32_t seqs);
 int ssb_kv_extend(const ssb_kv_cache* c, const int32_t* ids, const int32_t* counts, int32_t n, void* stream);
 
 /* Keys and values of new tokens into their pages, for one layer. Row r of k / v (16-bit elements, [rows, kv_heads, dim],
- * strides row_stride / head_stride in elements, dim contiguous) with starts[b] <= r < starts[b + 1] is token
+ * strides in elements, dim contiguous) with starts[b] <= r < starts[b + 1] is token
  * lengths[s] - (starts[b + 1] - starts[b]) + r - starts[b] of sequence s = ids ? ids[b] : b: the newest tokens, after
- * ssb_kv_extend. k_layer / v_layer: the layer's first element in the pool; page, head and token strides in elements.
- * A row whose page is missing or shared is dropped, with the error bit set. Strides are multiples of 8 elements. */
-int ssb_kv_write(const ssb_kv_cache* c, const uint16_t* k, const uint16_t* v, int64_t rows, int64_t k_row_stride,
-                 int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int32_t kv_heads, int32_t dim,
-                 const int32_t* starts, const int32_t* ids, int32_t n, uint16_t* k_layer, uint16_t* v_layer,
-                 int64_t page_stride, int64_t head_stride, int64_t token_stride, void* stream);
+ * ssb_kv_extend. k_layer / v_layer: the layer's first element in the pool. A row whose page is missing or shared is
+ * dropped, with the error bit set. Strides are multiples of 8 elements, pointers 16-byte aligned. */
+typedef struct ssb_kv_rows {
+  const uint16_t *k, *v;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, rows;
+  const int32_t *starts, *ids; /* [n + 1], [n] (nullable) */
+  uint16_t *k_layer, *v_layer;
+  int64_t page_stride, head_stride, token_stride;
+  int32_t n, kv_heads, dim;
+} ssb_kv_rows;
+int ssb_kv_write(const ssb_kv_cache* c, const ssb_kv_rows* r, void* stream);
 
 /* children[i] becomes a copy of parents[i] (i < n): full pages are shared (refs + 1), a partly filled last page is
  * copied to a fresh page (the lowest free ones, in the order of i), so that either can be extended. A child must be
@@ -487,8 +492,8 @@ int ssb_kv_compact(const ssb_kv_cache* c, void* stream);
 /* ---- attention over the paged cache. Token t of a sequence is visible to the query at position p when t <= p and
  * (window == 0 or p - t < window or t < sinks); o = sum softmax(scale * q . k) v over the visible tokens (fp32 scores,
  * softmax statistics and sums; the softmax weights are rounded to the inputs' type for the tensor cores), zero where
- * none is visible; lse (fp32, nullable) = log sum exp(scale * q . k), -inf there. q_type SSB_BF16 or SSB_F16, the cache
- * and out have the same. k / v: the layer's first key and value element in the pool, with page, head and token strides
+ * none is visible; lse (fp32, nullable) = log sum exp(scale * q . k), -inf there. type SSB_BF16 or SSB_F16: of q, the cache
+ * and out. k / v: the layer's first key and value element in the pool, with page, head and token strides
  * in elements (multiples of 8; 16-byte aligned); pages, page_size (any), table [table_rows, max_pages], lengths
  * [table_rows] as above; ids (nullable) maps batch row b to its table row (one out of range reads as empty and sets
  * SSB_ERR_SEQUENCE). What no query of the call sees is not read: its value may be anything. A NaN or infinity in the
@@ -498,24 +503,28 @@ int ssb_kv_compact(const ssb_kv_cache* c, void* stream);
  * ssb_attn_workspace bytes for the call's sizes (rows = all query tokens; 0: ws may be NULL), contents irrelevant between
  * calls; calls sharing it must not overlap.
  *
- * ssb_attn_decode: q [n, q_len, heads, dim] (strides in elements, multiples of 8), the q_len newest tokens of each
- * sequence (positions lengths - q_len ..; a position below 0 has no visible token). q_len * heads / kv_heads <= 128.
- * ssb_attn_prefill: ragged q [rows, heads, dim]; rows starts[b] <= r < starts[b + 1] are the newest tokens of
- * sequence b. out / lse are contiguous. */
-int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads, int32_t page_size,
-                       int32_t max_pages, int32_t window, int32_t sinks, int32_t prefill, int64_t* bytes);
-int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride,
-                    const void* k, const void* v, int64_t page_stride, int64_t head_stride, int64_t token_stride,
-                    int32_t n, int32_t q_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t page_size,
-                    int32_t pages, const int32_t* table, int32_t table_rows, int32_t max_pages, const int32_t* lengths,
-                    const int32_t* ids, int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
-                    int64_t ws_bytes, int32_t* err, void* stream);
-int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
-                     const void* v, int64_t page_stride, int64_t head_stride, int64_t token_stride, int64_t rows,
-                     const int32_t* starts, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim, int32_t page_size,
-                     int32_t pages, const int32_t* table, int32_t table_rows, int32_t max_pages, const int32_t* lengths,
-                     const int32_t* ids, int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
-                     int64_t ws_bytes, int32_t* err, void* stream);
+ * ssb_attn_decode: q [n, q_len, heads, dim], the q_len newest tokens of each sequence (positions lengths - q_len ..; a
+ * position below 0 has no visible token). q_len * heads / kv_heads <= 128.
+ * ssb_attn_prefill: ragged q [rows, heads, dim]; rows starts[b] <= r < starts[b + 1] are the newest tokens of sequence b;
+ * rows outside every sequence are not written. out and lse are contiguous. */
+typedef struct ssb_attn_args {
+  const void *q, *k, *v;
+  int64_t q_seq_stride, q_tok_stride, q_head_stride; /* elements, multiples of 8; q_seq_stride for decode only */
+  int64_t page_stride, head_stride, token_stride;    /* of k and v */
+  const int32_t *table, *lengths, *ids, *starts;     /* ids nullable; starts [n + 1] for prefill only */
+  void* out;
+  float* lse;
+  int32_t* err;
+  void* ws;
+  int64_t ws_bytes, rows;                            /* rows: query tokens, for prefill only */
+  int32_t type, n, q_len, heads, kv_heads, dim;      /* q_len for decode only */
+  int32_t page_size, pages, table_rows, max_pages, window, sinks;
+  float scale;
+} ssb_attn_args;
+/* Workspace of a call with these sizes (n, q_len or rows, heads, kv_heads, dim, page_size, max_pages, window, sinks). */
+int ssb_attn_workspace(const ssb_attn_args* a, int32_t prefill, int64_t* bytes);
+int ssb_attn_decode(const ssb_attn_args* a, void* stream);
+int ssb_attn_prefill(const ssb_attn_args* a, void* stream);
 
 #ifdef __cplusplus
 }

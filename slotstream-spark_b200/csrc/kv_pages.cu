@@ -532,27 +532,23 @@ extern "C" int ssb_kv_compact(const ssb_kv_cache* cc, void* stream) {
   return ssb_launch(k_compact_apply, dim3((unsigned)ssb_sm_count() * 8), dim3(COPY_T), 0, (cudaStream_t)stream, true, c);
 }
 
-extern "C" int ssb_kv_write(const ssb_kv_cache* cc, const uint16_t* k, const uint16_t* v, int64_t rows,
-                            int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                            int32_t kv_heads, int32_t dim, const int32_t* starts, const int32_t* ids, int32_t n,
-                            uint16_t* k_layer, uint16_t* v_layer, int64_t page_stride, int64_t head_stride,
-                            int64_t token_stride, void* stream) {
+extern "C" int ssb_kv_write(const ssb_kv_cache* cc, const ssb_kv_rows* w, void* stream) {
   Cache c;
   if (int rc = cache_of(cc, &c)) return rc;
-  SSB_CHECK_ARG(rows >= 0 && rows < (1ll << 31) && n >= 0 && kv_heads > 0 && dim > 0);
-  if (dim % 8) return SSB_EUNSUPPORTED;
-  if (rows == 0 || n == 0) return SSB_OK;
-  SSB_CHECK_ARG(k && v && starts && k_layer && v_layer);
-  const int64_t bits = k_row_stride | k_head_stride | v_row_stride | v_head_stride | page_stride | head_stride |
-                       token_stride;
+  SSB_CHECK_ARG(w && w->rows >= 0 && w->rows < (1ll << 31) && w->n >= 0 && w->kv_heads > 0 && w->dim > 0);
+  if (w->dim % 8) return SSB_EUNSUPPORTED;
+  if (w->rows == 0 || w->n == 0) return SSB_OK;
+  SSB_CHECK_ARG(w->k && w->v && w->starts && w->k_layer && w->v_layer);
+  const int64_t bits = w->k_row_stride | w->k_head_stride | w->v_row_stride | w->v_head_stride | w->page_stride |
+                       w->head_stride | w->token_stride;
   SSB_CHECK_ARG(bits % 8 == 0);
-  SSB_CHECK_ARG((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_layer | (uintptr_t)v_layer) & 15) == 0);
-  SSB_CHECK_ARG((int64_t)kv_heads * dim < (1ll << 30));
-  WriteArgs a{k, v, rows, k_row_stride, k_head_stride, v_row_stride, v_head_stride, kv_heads, dim, starts, ids, n,
-              k_layer, v_layer, page_stride, head_stride, token_stride, 0, 0};
-  while ((8ll << a.per_shift) < dim) ++a.per_shift;       // round-up reciprocal, for i < 2^31
-  a.per_mul = (uint32_t)((1ll << 32) * ((1ll << a.per_shift) - dim / 8) / (dim / 8) + 1);
+  SSB_CHECK_ARG((((uintptr_t)w->k | (uintptr_t)w->v | (uintptr_t)w->k_layer | (uintptr_t)w->v_layer) & 15) == 0);
+  SSB_CHECK_ARG((int64_t)w->kv_heads * w->dim < (1ll << 30));
+  WriteArgs a{w->k, w->v, w->rows, w->k_row_stride, w->k_head_stride, w->v_row_stride, w->v_head_stride, w->kv_heads, w->dim,
+              w->starts, w->ids, w->n, w->k_layer, w->v_layer, w->page_stride, w->head_stride, w->token_stride, 0, 0};
+  while ((8ll << a.per_shift) < w->dim) ++a.per_shift;    // round-up reciprocal, for i < 2^31
+  a.per_mul = (uint32_t)((1ll << 32) * ((1ll << a.per_shift) - w->dim / 8) / (w->dim / 8) + 1);
   static std::atomic<uint64_t> done{0};
   if (int rc = ssb_setup_kernel(done, "kv_write", k_write, 0)) return rc;
-  return ssb_launch(k_write, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, false, c, a);
+  return ssb_launch(k_write, dim3((unsigned)((w->rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, false, c, a);
 }

@@ -668,42 +668,40 @@ void reciprocal(int32_t d, uint32_t* mul, uint32_t* shift) {
 }
 
 // Checks and the fields that both entry points share.
-int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, int64_t page_stride,
-         int64_t head_stride, int64_t token_stride, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim,
-         int32_t page_size, int32_t pages, const int32_t* table, int32_t table_rows, int32_t max_pages,
-         const int32_t* lengths, const int32_t* ids, int32_t window, int32_t sinks, float scale, void* out, float* lse,
-         int32_t* err) {
-  SSB_CHECK_ARG(q_type == SSB_BF16 || q_type == SSB_F16);
-  SSB_CHECK_ARG(n >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && page_size > 0 && pages > 0 &&
-                table_rows > 0 && max_pages > 0 && window >= 0 && sinks >= 0 && scale > 0.f && scale <= 3.4e38f);
-  SSB_CHECK_ARG((int64_t)max_pages * page_size <= 0x7FFFFFFFll - 1024 && sinks <= 0x7FFFFFFF - 1024);
-  if (dim != 64 && dim != 128 && dim != 256) return SSB_EUNSUPPORTED;
-  SSB_CHECK_ARG((page_stride | head_stride | token_stride) % 8 == 0);
-  SSB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0);
-  a.q = (const uint16_t*)q;
-  a.k = (const uint16_t*)k;
-  a.v = (const uint16_t*)v;
-  a.sp = page_stride;
-  a.sh = head_stride;
-  a.st = token_stride;
-  a.n = n;
-  a.heads = heads;
-  a.kv_heads = kv_heads;
-  a.group = heads / kv_heads;
-  a.page_size = page_size;
-  a.pages = pages;
-  a.table = table;
-  a.table_rows = table_rows;
-  a.max_pages = max_pages;
-  a.lengths = lengths;
-  a.ids = ids;
-  a.window = window;
-  a.sinks = window ? sinks : 0;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = (uint16_t*)out;
-  a.lse = lse;
-  a.err = err;
-  reciprocal(page_size, &a.page_mul, &a.page_shift);
+int fill(Args& a, const ssb_attn_args& x) {
+  SSB_CHECK_ARG(x.type == SSB_BF16 || x.type == SSB_F16);
+  SSB_CHECK_ARG(x.n >= 0 && x.heads > 0 && x.kv_heads > 0 && x.heads % x.kv_heads == 0 && x.page_size > 0 && x.pages > 0 &&
+                x.table_rows > 0 && x.max_pages > 0 && x.window >= 0 && x.sinks >= 0 && x.scale > 0.f && x.scale <= 3.4e38f);
+  SSB_CHECK_ARG((int64_t)x.max_pages * x.page_size <= 0x7FFFFFFFll - 1024 && x.sinks <= 0x7FFFFFFF - 1024);
+  if (x.dim != 64 && x.dim != 128 && x.dim != 256) return SSB_EUNSUPPORTED;
+  SSB_CHECK_ARG((x.page_stride | x.head_stride | x.token_stride | x.q_tok_stride | x.q_head_stride) % 8 == 0);
+  SSB_CHECK_ARG((((uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v | (uintptr_t)x.out) & 15) == 0);
+  a.q = (const uint16_t*)x.q;
+  a.q_tok = x.q_tok_stride;
+  a.q_head = x.q_head_stride;
+  a.k = (const uint16_t*)x.k;
+  a.v = (const uint16_t*)x.v;
+  a.sp = x.page_stride;
+  a.sh = x.head_stride;
+  a.st = x.token_stride;
+  a.n = x.n;
+  a.heads = x.heads;
+  a.kv_heads = x.kv_heads;
+  a.group = x.heads / x.kv_heads;
+  a.page_size = x.page_size;
+  a.pages = x.pages;
+  a.table = x.table;
+  a.table_rows = x.table_rows;
+  a.max_pages = x.max_pages;
+  a.lengths = x.lengths;
+  a.ids = x.ids;
+  a.window = x.window;
+  a.sinks = x.window ? x.sinks : 0;
+  a.scale_log2 = x.scale * 1.4426950408889634f;
+  a.out = (uint16_t*)x.out;
+  a.lse = x.lse;
+  a.err = x.err;
+  reciprocal(x.page_size, &a.page_mul, &a.page_shift);
   reciprocal(a.group, &a.group_mul, &a.group_shift);
   return SSB_OK;
 }
@@ -713,70 +711,51 @@ int fill(Args& a, const void* q, int32_t q_type, const void* k, const void* v, i
 
 using namespace attn;
 
-extern "C" int ssb_attn_workspace(int32_t dim, int32_t n, int64_t rows, int32_t heads, int32_t kv_heads,
-                                  int32_t page_size, int32_t max_pages, int32_t window, int32_t sinks, int32_t prefill,
-                                  int64_t* bytes) {
-  SSB_CHECK_ARG(bytes && n >= 0 && rows >= 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0);
-  SSB_CHECK_ARG(rows * (heads / kv_heads) < (1ll << 30) && page_size > 0 && max_pages > 0 && window >= 0 && sinks >= 0);
-  if (dim != 64 && dim != 128 && dim != 256) return SSB_EUNSUPPORTED;
-  if (!prefill && n && rows % n) return SSB_EINVAL;
+extern "C" int ssb_attn_workspace(const ssb_attn_args* x, int32_t prefill, int64_t* bytes) {
+  SSB_CHECK_ARG(x && bytes && x->n >= 0 && x->kv_heads > 0 && x->heads > 0 && x->heads % x->kv_heads == 0);
+  SSB_CHECK_ARG(x->page_size > 0 && x->max_pages > 0 && x->window >= 0 && x->sinks >= 0 && x->rows >= 0 && x->q_len >= 0);
+  if (x->dim != 64 && x->dim != 128 && x->dim != 256) return SSB_EUNSUPPORTED;
   Args a = {};
-  a.n = n;
-  a.rows = rows;
-  a.heads = heads;
-  a.kv_heads = kv_heads;
-  a.group = heads / kv_heads;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.window = window;
-  a.sinks = window ? sinks : 0;
+  a.n = x->n;
+  a.heads = x->heads;
+  a.kv_heads = x->kv_heads;
+  a.group = x->heads / x->kv_heads;
+  a.page_size = x->page_size;
+  a.max_pages = x->max_pages;
+  a.window = x->window;
+  a.sinks = x->window ? x->sinks : 0;
   const int32_t some = 0;
   if (prefill) a.starts = &some;                     // only whether there are any matters here
-  else a.q_len = n ? (int32_t)(rows / n) : 0;
-  *bytes = n && rows ? workspace(a, dim) : 0;
+  else a.q_len = x->q_len;
+  a.rows = prefill ? x->rows : (int64_t)x->n * x->q_len;
+  SSB_CHECK_ARG(a.rows * a.group < (1ll << 30));
+  *bytes = a.n && a.rows ? workspace(a, x->dim) : 0;
   return SSB_OK;
 }
 
-extern "C" int ssb_attn_decode(const void* q, int32_t q_type, int64_t q_seq_stride, int64_t q_tok_stride,
-                               int64_t q_head_stride, const void* k, const void* v, int64_t page_stride,
-                               int64_t head_stride, int64_t token_stride, int32_t n, int32_t q_len, int32_t heads,
-                               int32_t kv_heads, int32_t dim, int32_t page_size, int32_t pages, const int32_t* table,
-                               int32_t table_rows, int32_t max_pages, const int32_t* lengths, const int32_t* ids,
-                               int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
-                               int64_t ws_bytes, int32_t* err, void* stream) {
+extern "C" int ssb_attn_decode(const ssb_attn_args* x, void* stream) {
   Args a = {};
-  if (int rc = fill(a, q, q_type, k, v, page_stride, head_stride, token_stride, n, heads, kv_heads, dim, page_size,
-                    pages, table, table_rows, max_pages, lengths, ids, window, sinks, scale, out, lse, err))
-    return rc;
-  SSB_CHECK_ARG(q_len >= 0 && (q_seq_stride | q_tok_stride | q_head_stride) % 8 == 0);
-  if ((int64_t)q_len * (heads / kv_heads) > 128) return SSB_EUNSUPPORTED;
-  if (n == 0 || q_len == 0) return SSB_OK;
-  SSB_CHECK_ARG(q && k && v && table && lengths && out);
-  a.q_seq = q_seq_stride;
-  a.q_tok = q_tok_stride;
-  a.q_head = q_head_stride;
-  a.q_len = q_len;
-  a.rows = (int64_t)n * q_len;
-  return launch_checked(a, dim, q_type == SSB_BF16, ws, ws_bytes, stream);
+  SSB_CHECK_ARG(x);
+  if (int rc = fill(a, *x)) return rc;
+  SSB_CHECK_ARG(x->q_len >= 0 && x->q_seq_stride % 8 == 0);
+  if ((int64_t)x->q_len * a.group > 128) return SSB_EUNSUPPORTED;
+  a.rows = (int64_t)x->n * x->q_len;
+  SSB_CHECK_ARG(a.rows * a.group < (1ll << 30));
+  if (a.rows == 0) return SSB_OK;
+  SSB_CHECK_ARG(x->q && x->k && x->v && x->table && x->lengths && x->out);
+  a.q_seq = x->q_seq_stride;
+  a.q_len = x->q_len;
+  return launch_checked(a, x->dim, x->type == SSB_BF16, x->ws, x->ws_bytes, stream);
 }
 
-extern "C" int ssb_attn_prefill(const void* q, int32_t q_type, int64_t q_tok_stride, int64_t q_head_stride,
-                                const void* k, const void* v, int64_t page_stride, int64_t head_stride,
-                                int64_t token_stride, int64_t rows, const int32_t* starts, int32_t n, int32_t heads,
-                                int32_t kv_heads, int32_t dim, int32_t page_size, int32_t pages, const int32_t* table,
-                                int32_t table_rows, int32_t max_pages, const int32_t* lengths, const int32_t* ids,
-                                int32_t window, int32_t sinks, float scale, void* out, float* lse, void* ws,
-                                int64_t ws_bytes, int32_t* err, void* stream) {
+extern "C" int ssb_attn_prefill(const ssb_attn_args* x, void* stream) {
   Args a = {};
-  if (int rc = fill(a, q, q_type, k, v, page_stride, head_stride, token_stride, n, heads, kv_heads, dim, page_size,
-                    pages, table, table_rows, max_pages, lengths, ids, window, sinks, scale, out, lse, err))
-    return rc;
-  SSB_CHECK_ARG(rows >= 0 && rows * (heads / kv_heads) < (1ll << 30) && (q_tok_stride | q_head_stride) % 8 == 0);
-  if (n == 0 || rows == 0) return SSB_OK;
-  SSB_CHECK_ARG(q && k && v && table && lengths && starts && out);
-  a.q_tok = q_tok_stride;
-  a.q_head = q_head_stride;
-  a.starts = starts;
-  a.rows = rows;
-  return launch_checked(a, dim, q_type == SSB_BF16, ws, ws_bytes, stream);
+  SSB_CHECK_ARG(x);
+  if (int rc = fill(a, *x)) return rc;
+  SSB_CHECK_ARG(x->rows >= 0 && x->rows * a.group < (1ll << 30));
+  if (x->n == 0 || x->rows == 0) return SSB_OK;
+  SSB_CHECK_ARG(x->q && x->k && x->v && x->table && x->lengths && x->starts && x->out);
+  a.starts = x->starts;
+  a.rows = x->rows;
+  return launch_checked(a, x->dim, x->type == SSB_BF16, x->ws, x->ws_bytes, stream);
 }

@@ -5,6 +5,7 @@ Launches go to torch's current CUDA stream, so the Python wrappers are CUDA-grap
 the caller provides every output and workspace.
 """
 import ctypes
+import struct
 from pathlib import Path
 
 import torch
@@ -23,7 +24,6 @@ DECODE_FUSED_TENSOR_CORES = 8
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
-_F32 = ctypes.c_float
 
 
 class KvCacheStruct(ctypes.Structure):
@@ -32,6 +32,11 @@ class KvCacheStruct(ctypes.Structure):
                 ("max_pages", _I32), ("lengths", _P), ("refs", _P), ("free_words", _P), ("table", _P), ("err", _P),
                 ("scratch", _P)]
 
+
+# ssb_attn_args and ssb_kv_rows of the C header, packed: a call with thirty ctypes arguments costs more host time (3.7 us)
+# than its launch.
+ATTN_ARGS = struct.Struct("@3P6q8P2q12if")
+KV_ROWS = struct.Struct("@2P5q4P3q3i")
 
 # name -> argtypes (every entry point returns int)
 SIGNATURES = {
@@ -87,15 +92,13 @@ SIGNATURES = {
     "ssb_gemm_dense": [_P, _I64, _I32, _P, _I32, _P, _I64, _P],
     "ssb_kv_scratch_ints": [_I32, _I32],
     "ssb_kv_extend": [_P, _P, _P, _I32, _P],
-    "ssb_kv_write": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P],
+    "ssb_kv_write": [_P, _P, _P],
     "ssb_kv_fork": [_P, _P, _P, _I32, _P],
     "ssb_kv_free": [_P, _P, _P, _P, _I32, _P],
     "ssb_kv_compact": [_P, _P],
-    "ssb_attn_workspace": [_I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
-    "ssb_attn_decode": [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
-                        _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
-    "ssb_attn_prefill": [_P, _I32, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32,
-                         _P, _I32, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _P],
+    "ssb_attn_workspace": [_P, _I32, _P],
+    "ssb_attn_decode": [_P, _P],
+    "ssb_attn_prefill": [_P, _P],
 }
 
 _lib = None

@@ -30,8 +30,11 @@ def workspace_bytes(head_dim: int, n: int, rows: int, heads: int, kv_heads: int,
     got = _WS.get(key)
     if got is None:
         b = ctypes.c_int64()
-        _lib.check(_lib.lib().ssb_attn_workspace(head_dim, n, rows, heads, kv_heads, page_size, max_pages, window, sinks,
-                                                 int(prefill), ctypes.byref(b)), "attention workspace")
+        if not prefill and n and rows % n:
+            raise ValueError(f"{rows} query tokens are no multiple of {n} sequences")
+        args = _lib.ATTN_ARGS.pack(*([0] * 18), rows, 0, n, rows // n if n else 0, heads, kv_heads, head_dim, page_size, 0, 0,
+                                   max_pages, window, sinks, 1.0)
+        _lib.check(_lib.lib().ssb_attn_workspace(args, int(prefill), ctypes.byref(b)), "attention workspace")
         if len(_WS) > 4096:
             _WS.clear()
         got = _WS[key] = b.value
@@ -49,7 +52,7 @@ def _bad_pages(q, k_pages, v_pages, dim, heads):
     return ValueError(f"{heads} query heads are no multiple of {k_pages.shape[1]} key heads")
 
 
-def _attend(call, what, q, heads, dim, n, tokens, starts, q_args, k_pages, v_pages, page_table, lengths, out, lse, scale,
+def _attend(call, what, q, heads, dim, n, q_len, tokens, starts, q_strides, k_pages, v_pages, page_table, lengths, out, lse, scale,
             window, sinks, ids, err, ws):
     """The checks, allocations and arguments that both entry points share."""
     tag = _TYPES.get(q.dtype)
@@ -67,8 +70,8 @@ def _attend(call, what, q, heads, dim, n, tokens, starts, q_args, k_pages, v_pag
             raise ValueError(f"ids must be a contiguous int32 vector of {n}")
     elif n > rows:
         raise ValueError(f"{n} sequences, but page_table has {rows} rows")
-    if window < 0 or sinks < 0:
-        raise ValueError("window and sinks must not be negative")
+    if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+        raise ValueError("window and sinks must not be negative, nor past 32 bits")
     if scale is None:
         scale = dim ** -0.5
     elif not 0 < scale < math.inf:
@@ -77,7 +80,7 @@ def _attend(call, what, q, heads, dim, n, tokens, starts, q_args, k_pages, v_pag
         raise ValueError("err must be one int32")
     shape = q.shape
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous, with q's shape and type")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:-1] or not lse.is_contiguous()):
@@ -89,10 +92,12 @@ def _attend(call, what, q, heads, dim, n, tokens, starts, q_args, k_pages, v_pag
     elif ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
         raise ValueError(f"ws must be a contiguous uint8 tensor of at least {need} bytes")
     p = _lib.ptr
-    rc = call(p(q), tag, *q_args, p(k_pages), p(v_pages), ks[0], ks[1], ks[2],
-              *((n, tokens // n if n else 0) if starts is None else (tokens, p(starts), n)), heads, ps[1], dim, ps[2], ps[0],
-              p(page_table), rows, max_pages, p(lengths), p(ids), window, sinks, scale, p(out), p(lse), p(ws), need, p(err),
-              _lib.stream())
+    args = _lib.ATTN_ARGS.pack(
+        p(q), p(k_pages), p(v_pages), *q_strides, ks[0], ks[1], ks[2], p(page_table), p(lengths), 0 if ids is None else p(ids),
+        0 if starts is None else p(starts), p(out), 0 if lse is None else p(lse), 0 if err is None else p(err),
+        0 if ws is None else p(ws), need, tokens, tag, n, q_len, heads, ps[1], dim, ps[2], ps[0], rows, max_pages, window, sinks,
+        scale)
+    rc = call(args, _lib.stream())
     if rc:
         _lib.check(rc, what)
     return out
@@ -107,7 +112,7 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, out=None, *, lse=None,
     if len(qs) != 4 or qs[3] != 1:
         raise ValueError("q must be [n, q_len, heads, head_dim] with a contiguous head_dim")
     n, q_len, heads, dim = q.shape
-    return _attend(_lib.lib().ssb_attn_decode, "attn_decode", q, heads, dim, n, n * q_len, None, qs[:3], k_pages, v_pages,
+    return _attend(_lib.lib().ssb_attn_decode, "attn_decode", q, heads, dim, n, q_len, n * q_len, None, qs[:3], k_pages, v_pages,
                    page_table, lengths, out, lse, scale, window, sinks, ids, err, ws)
 
 
@@ -122,5 +127,5 @@ def attn_prefill(q, k_pages, v_pages, page_table, lengths, starts, out=None, *, 
     if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector of at least one element")
     total, heads, dim = q.shape
-    return _attend(_lib.lib().ssb_attn_prefill, "attn_prefill", q, heads, dim, starts.shape[0] - 1, total, starts, qs[:2],
+    return _attend(_lib.lib().ssb_attn_prefill, "attn_prefill", q, heads, dim, starts.shape[0] - 1, 0, total, starts, (0, qs[0], qs[1]),
                    k_pages, v_pages, page_table, lengths, out, lse, scale, window, sinks, ids, err, ws)

@@ -120,11 +120,11 @@ class PagedKvCache:
         n = starts.numel() - 1
         if n < 0:
             raise ValueError("starts needs at least one element")
-        kl, vl, st = self._k[layer], self._v[layer], self._strides
-        rc = _lib.lib().ssb_kv_write(self._c, _lib.ptr(k), _lib.ptr(v), k.shape[0], ks[0], ks[1], vs[0], vs[1],
-                                     self.kv_heads, self.head_dim, _ids(starts, "starts"),
-                                     None if ids is None else _ids(ids, "ids", n), n, kl.data_ptr(), vl.data_ptr(), st[0],
-                                     st[1], st[2], _lib.stream())
+        p, st = _lib.ptr, self._strides
+        rows = _lib.KV_ROWS.pack(p(k), p(v), ks[0], ks[1], vs[0], vs[1], k.shape[0], _ids(starts, "starts"),
+                                 0 if ids is None else _ids(ids, "ids", n), self._k[layer].data_ptr(),
+                                 self._v[layer].data_ptr(), st[0], st[1], st[2], n, self.kv_heads, self.head_dim)
+        rc = _lib.lib().ssb_kv_write(self._c, rows, _lib.stream())
         _lib.check(rc, "kv write")
 
     def fork(self, parents, children):

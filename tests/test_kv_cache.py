@@ -73,6 +73,13 @@ def test_cache_lives_on_the_gpu():
         PagedKvCache(0, 1, 1, 16, 64, 1, 1)
 
 
+def _rows(**change):
+    f = dict(k=64, v=64, k_row=64, k_head=64, v_row=64, v_head=64, rows=1, starts=64, ids=0, kl=64, vl=64, sp=64, sh=64, st=64,
+             n=1, kv=1, dim=64)
+    f.update(change)
+    return _lib.KV_ROWS.pack(*f.values())
+
+
 def _c_cache(**change):
     f = dict(pool=4096, page_bytes=4096, pages=4, page_size=16, seqs=2, max_pages=3, lengths=64, refs=64, free_words=64,
              table=64, err=64, scratch=64)
@@ -92,7 +99,7 @@ def test_c_entry_refuses_a_bad_cache(change):
     assert L.ssb_kv_fork(p, 64, 64, 1, None) == _lib.SSB_EINVAL
     assert L.ssb_kv_free(p, 64, None, None, 1, None) == _lib.SSB_EINVAL
     assert L.ssb_kv_compact(p, None) == _lib.SSB_EINVAL
-    assert L.ssb_kv_write(p, 64, 64, 1, 64, 64, 64, 64, 1, 64, 64, None, 1, 64, 64, 64, 64, 64, None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(), None) == _lib.SSB_EINVAL
 
 
 def test_c_entry_counts_and_nulls():
@@ -104,19 +111,27 @@ def test_c_entry_counts_and_nulls():
     assert L.ssb_kv_extend(p, None, 64, 1, None) == _lib.SSB_EINVAL
     assert L.ssb_kv_fork(p, 64, None, 1, None) == _lib.SSB_EINVAL
     assert L.ssb_kv_free(p, 64, 64, None, 1, None) == _lib.SSB_EINVAL
-    assert L.ssb_kv_write(p, 64, 64, 1, 64, 64, 64, 64, 1, 60, 64, None, 1, 64, 64, 64, 64, 64, None) == _lib.SSB_EUNSUPPORTED
-    assert L.ssb_kv_write(p, 64, 64, 1, 60, 64, 64, 64, 1, 64, 64, None, 1, 64, 64, 64, 64, 64, None) == _lib.SSB_EINVAL
-    assert L.ssb_kv_write(p, 72, 64, 1, 64, 64, 64, 64, 1, 64, 64, None, 1, 64, 64, 64, 64, 64, None) == _lib.SSB_EINVAL
-    assert L.ssb_kv_write(p, 64, 64, 0, 64, 64, 64, 64, 1, 64, 64, None, 1, 64, 64, 64, 64, 64, None) == _lib.SSB_OK
+    assert L.ssb_kv_write(p, None, None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(dim=60), None) == _lib.SSB_EUNSUPPORTED
+    assert L.ssb_kv_write(p, _rows(k_row=60), None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(k=72), None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(starts=0), None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(rows=-1), None) == _lib.SSB_EINVAL
+    assert L.ssb_kv_write(p, _rows(rows=0), None) == _lib.SSB_OK
     assert L.ssb_kv_scratch_ints(0, 1) == _lib.SSB_EINVAL
 
 
-def _decode_args(**change):
-    f = dict(q=64, q_type=_lib.BF16, qs=64, qt=64, qh=64, k=64, v=64, sp=64, sh=64, st=64, n=1, q_len=1, heads=4, kv=2, dim=64,
-             ps=16, pages=4, table=64, rows=1, mp=3, lengths=64, ids=None, window=0, sinks=0, scale=1.0, out=64, lse=None,
-             ws=64, ws_bytes=0, err=None, stream=None)
+def _attn_args(**change):
+    f = dict(q=64, k=64, v=64, qs=64, qt=64, qh=64, sp=64, sh=64, st=64, table=64, lengths=64, ids=0, starts=64, out=64, lse=0,
+             err=0, ws=64, ws_bytes=0, total=1, q_type=_lib.BF16, n=1, q_len=1, heads=4, kv=2, dim=64, ps=16, pages=4, rows=1,
+             mp=3, window=0, sinks=0, scale=1.0)
     f.update(change)
-    return list(f.values())
+    return _lib.ATTN_ARGS.pack(*f.values())
+
+
+def test_packed_arguments_have_the_c_layout():
+    """The fields' order and alignment, and the sizes of the C structs without their padding at the end."""
+    assert _lib.ATTN_ARGS.size == 8 * 19 + 13 * 4 and _lib.KV_ROWS.size == 8 * 14 + 3 * 4
 
 
 @pytest.mark.parametrize("change,want", [
@@ -127,6 +142,22 @@ def _decode_args(**change):
     (dict(mp=1 << 28), _lib.SSB_EINVAL), (dict(window=-1), _lib.SSB_EINVAL), (dict(sinks=-1), _lib.SSB_EINVAL),
     (dict(st=63), _lib.SSB_EINVAL), (dict(qh=4), _lib.SSB_EINVAL), (dict(k=72), _lib.SSB_EINVAL),
     (dict(scale=-1.0), _lib.SSB_EINVAL), (dict(n=-1), _lib.SSB_EINVAL), (dict(n=0), _lib.SSB_OK), (dict(q_len=0), _lib.SSB_OK),
-    (dict(q=None, ws_bytes=1 << 40), _lib.SSB_EINVAL), (dict(ws=None, ws_bytes=1 << 40, mp=1 << 16), _lib.SSB_EINVAL)])
+    (dict(q=0, ws_bytes=1 << 40), _lib.SSB_EINVAL), (dict(ws=0, ws_bytes=1 << 40, mp=1 << 16), _lib.SSB_EINVAL)])
 def test_c_attention_refusals(change, want):
-    assert _lib.lib().ssb_attn_decode(*_decode_args(**change)) == want
+    assert _lib.lib().ssb_attn_decode(_attn_args(**change), None) == want
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(mp=1 << 16), _lib.SSB_EINVAL), (dict(total=-1), _lib.SSB_EINVAL), (dict(total=1 << 30), _lib.SSB_EINVAL),
+    (dict(starts=0), _lib.SSB_EINVAL), (dict(dim=32), _lib.SSB_EUNSUPPORTED), (dict(qt=4), _lib.SSB_EINVAL),
+    (dict(total=0), _lib.SSB_OK), (dict(n=0), _lib.SSB_OK)])
+def test_c_prefill_refusals(change, want):
+    assert _lib.lib().ssb_attn_prefill(_attn_args(**change), None) == want
+
+
+def test_c_null_arguments():
+    L, b = _lib.lib(), ctypes.c_int64()
+    assert L.ssb_attn_decode(None, None) == L.ssb_attn_prefill(None, None) == _lib.SSB_EINVAL
+    assert L.ssb_attn_workspace(None, 0, ctypes.byref(b)) == L.ssb_attn_workspace(_attn_args(), 0, None) == _lib.SSB_EINVAL
+    assert L.ssb_attn_workspace(_attn_args(mp=1 << 16), 0, ctypes.byref(b)) == _lib.SSB_OK and b.value > 0
+    assert L.ssb_attn_workspace(_attn_args(), 0, ctypes.byref(b)) == _lib.SSB_OK and b.value == 0
