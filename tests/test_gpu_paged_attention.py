@@ -10,11 +10,12 @@ pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
 
 
-def _cache(lengths, kv, dim, ps, dtype, seed=0, layers=2, layer=1, spare=3):
-    """Pages dealt at random, the slots past each length filled with NaN; returns strided k / v views and the table."""
+def _cache(lengths, kv, dim, ps, dtype, seed=0, layers=2, layer=1, spare=3, room=0):
+    """Pages dealt at random, the slots past each length filled with NaN; returns strided k / v views and the table, which
+    has room for ``room`` tokens a sequence."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     held = [-(-n // ps) for n in lengths]
-    pages, mp = sum(held) + spare, max(held + [1]) + 1
+    pages, mp = sum(held) + spare, max(held + [1, -(-room // ps)]) + 1
     pool = torch.full((pages, layers, 2, kv, ps, dim), float("nan"), dtype=dtype, device="cuda")
     order = np.random.default_rng(seed).permutation(pages)
     table = np.full((len(lengths), mp), -1, np.int32)
@@ -36,8 +37,8 @@ def _q(g, rows, heads, kv, dim, dtype):
     return both[:, :heads] * 1 if rows == 0 else both[:, :heads]
 
 
-def _decode(lengths, q_len, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0):
-    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed)
+def _decode(lengths, q_len, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0, room=0):
+    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed, room=room)
     n = len(lengths)
     q = _q(g, n * q_len, heads, kv, dim, dtype)
     lse = torch.full((n, q_len, heads), 7.0, device="cuda")
@@ -53,6 +54,15 @@ def _decode(lengths, q_len, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0
 @pytest.mark.parametrize("heads,kv", [(8, 1), (6, 2), (4, 4), (40, 2)])
 def test_decode_one_token(dtype, dim, heads, kv):
     _decode([1, 0, 17, 300, 1025], 1, heads, kv, dim, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,q_len", [(8, 2, 1), (24, 2, 1), (3, 1, 5)])
+def test_decode_split_over_the_gpu(dtype, dim, heads, kv, q_len):
+    """Tables with room for long sequences: the tiles are split evenly over the blocks and joined."""
+    assert workspace_bytes(dim, 5, 5 * q_len, heads, kv, 16, 40000 // 16) > 0
+    _decode([1, 0, 17, 300, 2049], q_len, heads, kv, dim, 16, dtype, room=40000)
 
 
 @pytest.mark.parametrize("ps", [1, 5, 8, 24, 100, 128])
@@ -80,9 +90,12 @@ def test_decode_many_sequences_and_a_long_one():
     _decode([20011], 1, 2, 1, 64, 32, HF)
 
 
-def _prefill(lengths, new, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0, ids=None):
-    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed)
+def _prefill(lengths, new, heads, kv, dim, ps, dtype, window=0, sinks=0, seed=0, ids=None, room=0):
+    k, v, table, lens, g = _cache(lengths, kv, dim, ps, dtype, seed, room=room)
     rows = sum(new)
+    if room or window:      # the tensor-core kernel's workspace, or none: which of the two kernels runs
+        big = workspace_bytes(dim, len(new), rows, heads, kv, ps, table.shape[1], window, sinks, prefill=True) > 0
+        assert big == (room > 0)
     q = _q(g, rows, heads, kv, dim, dtype)
     starts = torch.from_numpy(np.cumsum([0] + new).astype(np.int32)).cuda()
     lse = torch.full((rows, heads), 7.0, device="cuda")
@@ -101,15 +114,38 @@ def test_prefill_ragged(dtype, dim, heads, kv):
     _prefill([1, 37, 130, 257, 5], [1, 37, 129, 100, 0], heads, kv, dim, 16, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2), (8, 1), (5, 1), (32, 1)])
+@pytest.mark.parametrize("ps", [16, 24])
+def test_prefill_ragged_on_tcgen05(dtype, dim, heads, kv, ps):
+    """Tables with room for long prompts go to the tcgen05 kernel: pages in boxes (16) and row by row (24), groups that
+    divide its 128 rows and others."""
+    _prefill([1, 37, 130, 257, 5, 700], [1, 37, 129, 100, 0, 3], heads, kv, dim, ps, dtype, room=20000)
+
+
+@pytest.mark.parametrize("ps", [8, 32, 64, 128, 512])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prefill_boxes_of_every_page_size(ps, dim):
+    _prefill([600, 131], [300, 131], 4, 1, dim, ps, BF, room=20000)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (16, 4), (100, 0), (128, 300), (4000, 1)])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_prefill_window(window, sinks, dim):
-    _prefill([700, 300], [513, 300], 4, 2, dim, 24, BF, window, sinks)
+    _prefill([300, 110], [113, 110], 4, 2, dim, 24, BF, window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 4), (100, 0), (128, 300)])
+@pytest.mark.parametrize("dim,ps", [(64, 16), (128, 32), (256, 16), (128, 12)])
+def test_prefill_window_on_tcgen05(window, sinks, dim, ps):
+    _prefill([1500, 700], [900, 700], 16, 4, dim, ps, BF, window, sinks, room=1)
 
 
 @pytest.mark.parametrize("ps", [1, 7, 64, 200])
 def test_prefill_page_sizes_and_ids(ps):
     _prefill([300, 50, 411], [40, 411], 4, 1, 128, ps, BF, ids=[1, 2])
+    _prefill([300, 50, 411], [40, 411], 4, 1, 128, ps, BF, ids=[1, 2], room=20000)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
@@ -127,20 +163,38 @@ def test_scores_that_rise_or_fall_along_the_cache(dim, falling):
     q = _q(g, new, heads, kv, dim, BF)
     q[::3] *= 0.01
     starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
-    lse = torch.empty(new, heads, device="cuda")
-    out = attn_prefill(q, k, v, table, lens, starts, lse=lse)
-    assert_attention(out, lse, attention(q, k, v, table, lens, [new]))
-    out = attn_decode(q[-3:][None], k, v, table, lens, lse=lse[None, -3:])
-    assert_attention(out[0], lse[-3:], attention(q[-3:], k, v, table, lens, [3]))
+    lse, ref = torch.empty(new, heads, device="cuda"), attention(q, k, v, table, lens, [new])
+    wide = torch.cat([table, torch.full((1, 1500), -1, dtype=torch.int32, device="cuda")], 1)   # room for 25,000 tokens
+    for t in (table, wide):                                                                     # both kernels
+        out = attn_prefill(q, k, v, t, lens, starts, lse=lse)
+        assert_attention(out, lse, ref)
+        out = attn_decode(q[-3:][None], k, v, t, lens, lse=lse[None, -3:])
+        assert_attention(out[0], lse[-3:], [x[-3:] for x in ref])
 
 
 def test_prefill_long_context_few_rows():
     _prefill([9001], [3], 4, 2, 128, 32, BF)
-    _prefill([6000], [17], 16, 2, 256, 16, HF, 5000, 8)
+    _prefill([6000], [17], 16, 2, 256, 16, HF, 5000, 8, room=1)
 
 
-def test_prefill_more_queries_than_tokens_sees_nothing():
-    _prefill([3, 0], [8, 4], 4, 2, 64, 16, BF)
+@pytest.mark.parametrize("room", [0, 20000])
+def test_prefill_more_queries_than_tokens_sees_nothing(room):
+    _prefill([3, 0], [8, 4], 4, 2, 64, 16, BF, room=room)
+
+
+@pytest.mark.parametrize("room", [0, 20000])
+def test_prefill_missing_page_reads_as_zeros_and_is_reported(room):
+    k, v, table, lens, g = _cache([700], 1, 128, 16, BF, room=room)
+    q = _q(g, 200, 4, 1, 128, BF)
+    starts = torch.tensor([0, 200], dtype=torch.int32, device="cuda")
+    bad = table.clone()
+    bad[0, 5], bad[0, 40] = -1, 10 ** 6
+    err, lse = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty(200, 4, device="cuda")
+    out = attn_prefill(q, k, v, bad, lens, starts, lse=lse, err=err)
+    assert int(err.item()) == 128
+    none = torch.zeros_like(k[:1])
+    bad[0, 5] = bad[0, 40] = k.shape[0]
+    assert_attention(out, lse, attention(q, torch.cat([k, none]), torch.cat([v, none]), bad, lens, [200]))
 
 
 def test_ids_choose_table_rows_and_bad_ids_read_as_empty():
