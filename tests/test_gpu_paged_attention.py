@@ -223,6 +223,29 @@ def test_missing_page_reads_as_zeros_and_is_reported():
     assert bool(((out[0].double() - ref[0]).abs() <= ref[2]).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("room", [0, 20000])
+def test_other_orders_of_the_cache_and_of_the_queries(dim, room):
+    """Token-major pages [pages, page, heads, dim], pages apart by more than their size, and head-major queries."""
+    k, v, table, lens, g = _cache([300, 77], 2, dim, 16, BF, room=room)
+    q = _q(g, 250, 8, 2, dim, BF)
+    starts = torch.tensor([0, 200, 250], dtype=torch.int32, device="cuda")
+    lse = torch.empty(250, 8, device="cuda")
+    ref = attention(q, k, v, table, lens, [200, 50])
+    wide = torch.zeros(k.shape[0], 3, 16, 2, dim, dtype=BF, device="cuda")
+    wide[:, 0], wide[:, 2] = k.transpose(1, 2), v.transpose(1, 2)
+    k2, v2 = wide[:, 0].transpose(1, 2), wide[:, 2].transpose(1, 2)
+    q2 = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert not k2.is_contiguous() and not q2.is_contiguous()
+    for kk, vv, qq in ((k2, v2, q), (k, v, q2), (k2, v2, q2)):
+        out = attn_prefill(qq, kk, vv, table, lens, starts, lse=lse)
+        assert out.is_contiguous()
+        assert_attention(out, lse, ref)
+        out = attn_decode(qq[[199, 249]][:, None].contiguous() if qq is q else qq[[199, 249]][:, None], kk, vv, table, lens)
+        o, _, tol, _ = ref
+        assert bool(((out[:, 0].double() - o[[199, 249]]).abs() <= tol[[199, 249]]).all())
+
+
 def test_pages_behind_the_window_are_not_read():
     """The pages between the sinks and the window may be gone (-1): no error, the same result."""
     k, v, table, lens, g = _cache([700], 2, 128, 16, BF)
