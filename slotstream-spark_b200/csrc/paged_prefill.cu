@@ -22,7 +22,9 @@
 // cycles for 32 columns' worth of work (operands read from shared memory), so the products of a pair of tiles take 2570
 // cycles per 128 tokens instead of 2050; single-buffered tiles of 128, where each S waits for the product before it, took
 // 4600 (32K tokens, 32 heads, 8 key heads, window 4096: 2.16 ms against 1.91, 1.08 PFLOP/s). At size 256 two chunks of 2,048
-// tokens after 14K and 3K take 0.61 ms (1.05 PFLOP/s), bound by the shared memory's bandwidth: 192 KB a tile and row tile.
+// tokens after 14K and 3K take 0.61 ms (1.05 PFLOP/s): each tile brings 64 KB of K and V for one row tile, 8 TB/s out of L2 through a
+// ring of only five slots, and shared memory moves 192 KB for it. Without the exponentials it takes as long, with half of
+// Q K^T left out 0.52 (10 TB/s); the scores of two tiles in one instruction of 128 columns hold two slots at once: 0.68.
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
