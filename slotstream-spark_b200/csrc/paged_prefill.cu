@@ -32,6 +32,8 @@
 // pieces in order, so the outcome does not depend on who took which.
 #include "paged_attn.cuh"
 
+#include <type_traits>
+
 #include "affine.cuh"
 #include "tc_common.cuh"
 
@@ -252,9 +254,13 @@ SSB_DEV bool wait(uint64_t* bar, uint32_t parity) {
     else if (t - t0 > SSB_WAIT_NS) return false;
   }
 }
-// The same by a whole warp that goes on to warp-wide TMEM instructions: the lanes may leave the wait one by one, and the
-// vote brings them together again.
+// The same by a whole warp that goes on to warp-wide instructions (TMEM, shuffles): the lanes may leave the wait one by one,
+// and the vote brings them together again, so that either all of them go on or all of them give up. A full-mask instruction
+// that some lanes have given up on would never end.
 SSB_DEV bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
+
+using OneLane = std::false_type;
+using WholeWarp = std::true_type;
 
 // Shared-memory descriptors as (low word, constant high word): moving inside a tile adds to the low word only. That keeps
 // the one thread that issues the products off the critical path -- with descriptors built from scratch it took about 100
@@ -396,10 +402,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
   const uint32_t tmem = *tmem_slot;
   auto give_up = [&] { atomicExch(failed, 1); };
   int un = 0;                                       // units this thread has seen
-  // The next unit, or false at the end of the list (or when a wait gave up).
-  auto next_unit = [&](Unit& u) {
+  // The next unit, or false at the end of the list (or when a wait gave up). `by_warp`: called by all lanes of a warp.
+  auto next_unit = [&](Unit& u, auto by_warp) {
     const int s = un & 1;
-    if (!wait(u_full + s, (un >> 1) & 1)) {
+    if (!(by_warp.value ? warp_wait(u_full + s, (un >> 1) & 1) : wait(u_full + s, (un >> 1) & 1))) {
       give_up();
       return false;
     }
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     uint32_t kv = 0, qn = 0, tn = 0;                // slots, units and tiles so far
     bool ok = true;
     auto need = [&](uint64_t* b, uint32_t parity) { ok = ok && wait(b, parity); };
-    while (ok && next_unit(u)) {
+    while (ok && next_unit(u, OneLane())) {
       if (scores) need(q_full, qn++);
 #pragma unroll 1
       for (int i = u.i0; i < u.i1 && ok; ++i, ++tn, kv += 2) {
@@ -490,9 +496,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       ++given;
       return true;
     };
-    ok = give_unit();
-    while (ok && next_unit(u)) {
-      if (!give_unit()) {
+    // Every decision to go on or to give up is a vote of the warp: the shuffles below need all of its lanes.
+    ok = __all_sync(0xFFFFFFFFu, give_unit());
+    while (ok && next_unit(u, WholeWarp())) {
+      if (!__all_sync(0xFFFFFFFFu, give_unit())) {
         ok = false;
         break;
       }
@@ -500,7 +507,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
       const int p = u.len - u.q, p_lo = p + u.r0 / a.group, p_hi = p + (u.r0 + u.rows - 1) / a.group;
       const uint16_t *kh = a.k + u.h * a.sh, *vh = a.v + u.h * a.sh;
       const int32_t* trow = a.table + (int64_t)max(u.row, 0) * a.max_pages;
-      if (qn && !wait(q_empty, (qn - 1) & 1)) {
+      if (qn && !warp_wait(q_empty, (qn - 1) & 1)) {
         ok = false;
         break;
       }
@@ -582,8 +589,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
           const uint32_t at = pt * w.page_rows * (D * 2);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (ok && kv >= SLOTS && !wait(empty + kv % SLOTS, kv / SLOTS - 1)) ok = false;
-            if (!ok) break;
+            if (kv >= SLOTS && !warp_wait(empty + kv % SLOTS, kv / SLOTS - 1)) {
+              ok = false;
+              break;
+            }
             uint64_t* bar_full = full + kv % SLOTS;
             if (pt >= n_boxes) {
               mbar_arrive(bar_full);
@@ -604,12 +613,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
         } else {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (ok && kv >= SLOTS && !ready(empty + kv % SLOTS, kv / SLOTS - 1)) {
+            if (kv >= SLOTS && !__all_sync(0xFFFFFFFFu, ready(empty + kv % SLOTS, kv / SLOTS - 1))) {
               cp_async_wait_all();                     // nothing to issue: hand over what is on its way first
               hand_over(kv);
-              ok = wait(empty + kv % SLOTS, kv / SLOTS - 1);
+              if (!warp_wait(empty + kv % SLOTS, kv / SLOTS - 1)) {
+                ok = false;
+                break;
+              }
             }
-            if (!ok) break;
             const uint32_t dst = smem_u32(ring + (kv % SLOTS) * C::SLOT);
             const uint16_t* base = x ? vh : kh;
             constexpr int RPP = 32 / CPR > 0 ? 32 / CPR : 1, PASSES = (T / 4) * CPR / 32;
@@ -647,7 +658,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     Unit u;
     uint32_t tn = 0;
     bool ok = true;
-    while (ok && next_unit(u)) {
+    while (ok && next_unit(u, WholeWarp())) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
       const int pos = p + min(f0 + row, last) / a.group;       // rows past the last: zero queries, never written
