@@ -42,6 +42,7 @@ extern "C" {
 #define SSB_ERR_SEQUENCE 64    /* a sequence id out of range or named twice, a bad count, a fork onto a held sequence */
 #define SSB_ERR_PAGE_RANGE 128 /* a page id outside the pool: its tokens read as zeros, writes to it are dropped */
 #define SSB_ERR_SHARED_PAGE 256 /* new tokens would go into a page that another sequence holds too */
+#define SSB_ERR_NO_ROOM 512    /* rows of a sequence whose last ssb_kv_extend was refused (dropped) */
 
 /* ---- dtype tags for activations */
 #define SSB_BF16 0
@@ -436,8 +437,8 @@ int ssb_gemv_dense(const void* x, int32_t x_dtype, int64_t rows, const uint16_t*
  * s, or -1. refs[p] counts the table entries that hold page p; bit p % 32 of free_words[p / 32] is set exactly while
  * refs[p] is 0 (bits past `pages` are 0). lengths[s] = tokens of sequence s. All state is caller-owned device memory,
  * read and changed in stream order: no call waits for the host, so calls can be captured. err gets SSB_ERR_* bits.
- * scratch: int32 [ssb_kv_scratch_ints(pages, seqs)], contents irrelevant between calls; calls sharing a cache must not
- * overlap. seqs <= 65536, pages <= 2^20, page_bytes a multiple of 16, pool 16-byte aligned. */
+ * scratch: int32 [ssb_kv_scratch_ints(pages, seqs)], set to zero once by the caller and left alone afterwards (it holds
+ * which sequences wait for room); calls sharing a cache must not overlap. seqs <= 65536, pages <= 2^20, page_bytes a multiple of 16, pool 16-byte aligned. */
 typedef struct ssb_kv_cache {
   void* pool;
   int64_t page_bytes;
@@ -456,14 +457,15 @@ int ssb_kv_scratch_ints(int32_t pages, int32_t seqs);
 /* lengths[ids[i]] += counts[i] for i < n, with pages for the new tokens: the entries that a sequence lacks get the
  * lowest free pages, in the order of i and then of the entries. All or nothing: with too few free pages, a row that
  * would pass max_pages, a bad or repeated id, a negative count, or new tokens in a page that refs says is shared,
- * nothing changes and the error bit is set. */
+ * nothing changes and the error bit is set; ssb_kv_write then drops the rows of every sequence that the call named with
+ * new tokens, until a later call has made room for it. */
 int ssb_kv_extend(const ssb_kv_cache* c, const int32_t* ids, const int32_t* counts, int32_t n, void* stream);
 
 /* Keys and values of new tokens into their pages, for one layer. Row r of k / v (16-bit elements, [rows, kv_heads, dim],
  * strides in elements, dim contiguous) with starts[b] <= r < starts[b + 1] is token
  * lengths[s] - (starts[b + 1] - starts[b]) + r - starts[b] of sequence s = ids ? ids[b] : b: the newest tokens, after
- * ssb_kv_extend. k_layer / v_layer: the layer's first element in the pool. A row whose page is missing or shared is
- * dropped, with the error bit set. Strides are multiples of 8 elements, pointers 16-byte aligned. */
+ * ssb_kv_extend. k_layer / v_layer: the layer's first element in the pool. A row whose page is missing or shared, or
+ * whose sequence's last ssb_kv_extend was refused, is dropped, with the error bit set. Strides are multiples of 8 elements, pointers 16-byte aligned. */
 typedef struct ssb_kv_rows {
   const uint16_t *k, *v;
   int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, rows;

@@ -26,11 +26,15 @@ struct Cache {
 };
 
 // scratch: [0] copies, [1] rows to share, [2] live pages of a compaction; then src / dst of the copies, a page list, two
-// arrays of `seqs` (per-sequence counts), and one of pages + 2 seqs (counts of 32 table entries each).
+// arrays of `seqs` (per-sequence counts), one of pages + 2 seqs (counts of 32 table entries each), and a bit per sequence
+// that its last extend was refused. Only these bits are kept from call to call.
 struct Scratch {
   int32_t *head, *src, *dst, *list, *num, *num2, *part;
+  uint32_t* refused;
 };
-__host__ __device__ inline int64_t scratch_ints(int64_t pages, int64_t seqs) { return 8 + 4 * pages + 4 * seqs; }
+__host__ __device__ inline int64_t scratch_ints(int64_t pages, int64_t seqs) {
+  return 8 + 4 * pages + 4 * seqs + (seqs + 31) / 32;
+}
 SSB_DEV Scratch scratch_of(const Cache& c) {
   Scratch s;
   s.head = c.scratch;
@@ -40,6 +44,7 @@ SSB_DEV Scratch scratch_of(const Cache& c) {
   s.num = s.list + c.pages;
   s.num2 = s.num + c.seqs;
   s.part = s.num2 + c.seqs;
+  s.refused = (uint32_t*)(s.part + c.pages + 2 * c.seqs);
   return s;
 }
 
@@ -115,6 +120,9 @@ SSB_DEV bool seen_before(uint32_t* bitmap, int s) {
 
 // Allocation: the table entries that the new tokens fall into, in runs of 32 (a warp each), are counted where they lack a
 // page, the counts are scanned, and the lowest free pages dealt out in that order.
+// A refused call leaves lengths as they are, so rows written next would land on the newest tokens that are there, in pages
+// that nobody shares. Hence the sequences that it was to give room are marked until an extend has made room for them, and
+// k_write drops the rows of marked ones: a step that extends and writes (in a captured graph, say) need not look in between.
 __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __restrict__ ids,
                                                    const int32_t* __restrict__ counts, int n) {
   extern __shared__ uint32_t bitmap[];
@@ -125,6 +133,13 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
   for (int i = threadIdx.x; i < (c.seqs + 31) >> 5; i += PLAN_T) bitmap[i] = 0;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
+  auto refuse = [&](int why) {
+    for (int i = threadIdx.x; i < n; i += PLAN_T) {
+      const int s = ids[i];
+      if (s >= 0 && s < c.seqs && counts[i] != 0) atomicOr(&sc.refused[s >> 5], 1u << (s & 31));
+    }
+    if (threadIdx.x == 0) set_err(c.err, why);
+  };
   // entries of each sequence, its first run, and where in the table they begin; in shared memory where the call is small
   __shared__ int s_num[PLAN_T], s_run[PLAN_T];
   __shared__ int64_t s_at[PLAN_T];
@@ -159,10 +174,7 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
   }
   if (runs > most && threadIdx.x == 0) atomicOr(&bad, SSB_ERR_NO_PAGES);
   __syncthreads();
-  if (bad) {
-    if (threadIdx.x == 0) set_err(c.err, bad);
-    return;
-  }
+  if (bad) return refuse(bad);
   // run r: its sequence's table entry for this lane (nullptr past the last)
   auto entry_of = [&](int r) -> int32_t* {
     int lo = 0, hi = n;                                // the last i with run[i] <= r
@@ -195,14 +207,8 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
     need += total;
   }
   __syncthreads();
-  if (bad) {
-    if (threadIdx.x == 0) set_err(c.err, bad);
-    return;
-  }
-  if (!take_pages(c, need, sc.list, part)) {
-    if (threadIdx.x == 0) set_err(c.err, SSB_ERR_NO_PAGES);
-    return;
-  }
+  if (bad) return refuse(bad);
+  if (!take_pages(c, need, sc.list, part)) return refuse(SSB_ERR_NO_PAGES);
   for (int r = warp; r < runs; r += PLAN_T / 32) {
     int32_t* e = entry_of(r);
     const bool lacks = e && *e < 0;
@@ -210,7 +216,11 @@ __global__ void __launch_bounds__(PLAN_T) k_extend(Cache c, const int32_t* __res
     if (lacks) *e = sc.list[sc.part[r] + __popc(m & lanemask_lt())];
   }
   __syncthreads();                                     // entries are found through the old lengths
-  for (int i = threadIdx.x; i < n; i += PLAN_T) c.lengths[ids[i]] += counts[i];
+  for (int i = threadIdx.x; i < n; i += PLAN_T) {
+    const int s = ids[i];
+    c.lengths[s] += counts[i];
+    if (sc.refused[s >> 5] >> (s & 31) & 1) atomicAnd(&sc.refused[s >> 5], ~(1u << (s & 31)));
+  }
 }
 
 __global__ void __launch_bounds__(PLAN_T) k_fork_plan(Cache c, const int32_t* __restrict__ parents,
@@ -437,6 +447,10 @@ __global__ void __launch_bounds__(256) k_write(Cache c, WriteArgs a) {
   const int s = a.ids ? a.ids[lo] : lo;
   if (s < 0 || s >= c.seqs) {
     if (lane == 0) set_err(c.err, SSB_ERR_SEQUENCE);
+    return;
+  }
+  if (scratch_of(c).refused[s >> 5] >> (s & 31) & 1) {   // no room was made for the row
+    if (lane == 0) set_err(c.err, SSB_ERR_NO_ROOM);
     return;
   }
   const int64_t pos = c.lengths[s] - (b1 - b0) + (r - b0);

@@ -14,7 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libslotstream_b200.so"
 
 SSB_OK, SSB_EINVAL, SSB_EUNSUPPORTED, SSB_ENODEVICE, SSB_ETOOBIG, SSB_ETIMEDOUT = 0, -1, -2, -3, -4, -5
 ERR_EXPERT_RANGE, ERR_UNMAPPED, ERR_SLOT_RANGE, ERR_MISALIGNED, ERR_TIMEOUT = 1, 2, 4, 8, 16
-ERR_NO_PAGES, ERR_SEQUENCE, ERR_PAGE_RANGE, ERR_SHARED_PAGE = 32, 64, 128, 256
+ERR_NO_PAGES, ERR_SEQUENCE, ERR_PAGE_RANGE, ERR_SHARED_PAGE, ERR_NO_ROOM = 32, 64, 128, 256, 512
 BF16, F32, F16 = 0, 1, 2
 ROUTER_ROUND_BF16, ROUTER_SHARED_GATE = 1, 2
 DECODE_PDL = 1

@@ -8,7 +8,9 @@ contiguous run of bytes to copy, and ``k(layer)`` / ``v(layer)`` are strided vie
 
 All state is device memory and every call only launches on the current stream: nothing waits for the host, and the calls
 can be captured in a CUDA graph. What the device finds wrong -- no free pages, a bad or repeated sequence, a shared page
-about to be written -- leaves the state as it was and sets a bit in ``err``; ``check()`` reads it (and waits for it).
+about to be written -- leaves the state as it was and sets a bit in ``err``; ``check()`` reads it (and waits for it). After
+an ``extend`` that was refused, ``write`` drops the rows of the sequences that it named until an ``extend`` has made room for
+them, so that a step need not look in between; the attention of that step then sees the tokens of before.
 
 A decode step: ``extend(ids, counts)`` once (lengths grow, pages are allocated), then per layer ``write(layer, k, v,
 starts, ids)``, ``attn_decode(q, cache.k(layer), cache.v(layer), cache.table, cache.lengths, ids=ids)`` and the MoE layer.
@@ -23,7 +25,8 @@ _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ERRORS = {_lib.ERR_NO_PAGES: "not enough free pages, or a table row is full",
            _lib.ERR_SEQUENCE: "a sequence id out of range or repeated, a bad count, or a fork onto a held sequence",
            _lib.ERR_PAGE_RANGE: "a missing page or one outside the pool",
-           _lib.ERR_SHARED_PAGE: "new tokens in a page that another sequence holds too"}
+           _lib.ERR_SHARED_PAGE: "new tokens in a page that another sequence holds too",
+           _lib.ERR_NO_ROOM: "rows for a sequence whose last extend was refused, which were dropped"}
 
 
 def state_ints(pages: int, seqs: int, max_pages: int) -> int:
@@ -74,7 +77,7 @@ class PagedKvCache:
         ints = L.ssb_kv_scratch_ints(self.pages, seqs)
         if ints < 0:
             raise ValueError(f"a cache has at most 2^20 pages and 65536 sequences, got {self.pages} and {seqs}")
-        self.scratch = torch.empty(ints, dtype=torch.int32, device=pool.device)
+        self.scratch = torch.zeros(ints, dtype=torch.int32, device=pool.device)
         p = _lib.ptr
         self._struct = _lib.KvCacheStruct(p(pool), pool[0].numel() * pool.element_size(), self.pages, self.page_size, seqs,
                                           self.max_pages, p(self.lengths), p(self.refs), p(self.free_words),
@@ -87,6 +90,7 @@ class PagedKvCache:
     def reset(self):
         """Every sequence empty, every page free, no error."""
         self.state.zero_()
+        self.scratch.zero_()
         self.table.fill_(-1)
         self.free_words.fill_(-1)
         if self.pages % 32:
@@ -100,7 +104,8 @@ class PagedKvCache:
         return self._v[layer]
 
     def extend(self, ids, counts):
-        """lengths[ids[i]] += counts[i] (int32 vectors on the device), with the lowest free pages for the new tokens."""
+        """lengths[ids[i]] += counts[i] (int32 vectors on the device), with the lowest free pages for the new tokens; all of
+        them or, when something is wrong, none."""
         n = ids.numel()
         if n > self.seqs:
             raise ValueError(f"{n} sequences named, the cache has {self.seqs}")
