@@ -11,8 +11,9 @@
 //
 // A block has NW warps that work alone: each walks every NW-th sub-tile of TW tokens through its own ring of cp.async
 // units (no block barrier inside an item), and the warps' (max, sum, accumulator) are joined through shared
-// memory at the end of the item. p is rounded to the inputs' type for the second product (relative 2^-8 for bf16,
-// 2^-11 for fp16, as the library's other tensor-core inputs); its sum is taken before the rounding, in fp32.
+// memory at the end of the item. p is rounded to the inputs' type for the second product (half an ulp: relative 2^-8 for bf16,
+// 2^-11 for fp16 down to 2^-29 of the largest weight and 2^-40 of that one below, see below_max; as the library's other
+// tensor-core inputs); its sum is taken before the rounding, in fp32.
 #include "paged_attn.cuh"
 
 #include <cooperative_groups.h>
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(NW * 32, BLOCKS_PER_SM) k_attn_rows(Args a, in
           v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
-          top[n][y] = fmaxf(v, m[n][y]);
+          top[n][y] = fmaxf(below_max<E, 0>(v), m[n][y]);
           up |= top[n][y] != m[n][y];
         }
       if (__any_sync(0xFFFFFFFFu, up)) {

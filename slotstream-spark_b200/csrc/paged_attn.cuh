@@ -7,6 +7,8 @@
 // blocks leaves (max, sum, accumulator) pieces in the workspace, which k_attn_join sums in block order. The split
 // depends on the lengths alone, so results do not change from run to run.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "registry.h"
 
@@ -106,6 +108,17 @@ SSB_DEV float ex2(float x) {
   return y;
 }
 constexpr float LN2 = 0.6931471805599453f;
+
+// The weights p = 2^(s - m) are rounded to E for the second product. fp16 has no normal numbers below 2^-14, and a long context
+// is made of weights that small as soon as one token stands out by 10 nats; so for it m is kept 15 - STEP below the maximum
+// (STEP: how far the maximum may run ahead of m), which puts the largest weight at 2^15, just inside the type. o and l carry
+// the factor alike and m + log2 l does not see it. Weights then keep 11 bits down to 2^(STEP - 29) of the largest and an
+// absolute 2^(STEP - 40) of it below. Where scores are so large that m would lose the 15 to rounding, m is the maximum itself.
+template <typename E, int STEP>
+SSB_DEV float below_max(float max) {
+  constexpr float LIFT = std::is_same<E, __half>::value ? 15.f - STEP : 0.f;
+  return LIFT == 0.f || fabsf(max) >= 1048576.f ? max : max - LIFT;
+}
 
 // csrc/paged_prefill.cu
 int64_t prefill_workspace(int dim, int n, int64_t rows, int heads, int kv_heads);

@@ -9,8 +9,11 @@
 // of S for each: the S of the next tile is computed under the softmax of this one, so neither waits for the latency of the other
 // (about 350 cycles from an instruction's issue to a waiting thread).
 //
-// The running maximum is only raised when a row's maximum grows by more than 2^8 (log2 domain): p stays below 2^8, which
-// both types and the fp32 sums hold with the same relative precision, and rescaling the accumulator in TMEM becomes rare.
+// The running maximum is only raised when a row's maximum grows by more than STEP (log2 domain; a published form of the online
+// softmax): p stays below 2^STEP times what it is for the maximum itself, and rescaling the accumulator in TMEM becomes rare.
+// bf16 holds all these weights with 8 bits; for fp16 see below_max, which leaves 11 bits down to 2^-21 of the largest weight
+// and an error of 2^-32 of it below. A smaller STEP would leave more and costs time (fp16, 32K tokens, window 4096, 32 / 8
+// heads of 128: 2.01 ms at 8, 2.13 at 6, 2.23 at 4, 2.63 at 0; without the shift 1.99).
 //
 // Warps: NT groups of four for the softmax (one thread per row; TMEM lane = row), four that bring Q, K and V into
 // 128-byte-swizzled tiles (TMA boxes where pages allow, else row by row with cp.async; rows that no query sees become zeros) and
@@ -32,8 +35,6 @@
 // pieces in order, so the outcome does not depend on who took which.
 #include "paged_attn.cuh"
 
-#include <type_traits>
-
 #include "affine.cuh"
 #include "tc_common.cuh"
 
@@ -51,6 +52,7 @@ struct Cfg {
   static_assert(NBUF >= 2 && NT * NBUF <= 6, "TMEM");
 };
 constexpr int PLAN_T = 1024, LAG = 1;
+constexpr int STEP = 8;          // how far (log2) a row's maximum runs ahead of the one that its weights are taken against
 
 struct __align__(16) Unit {
   int b, h, r0, rows;          // sequence, key head, first flat row, rows
@@ -690,11 +692,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
           for (int y = 0; y < 4; ++y)
             m4[y] = x + 4 + y < T ? fmaxf(m4[y], fmaxf(v[x + y], v[x + 4 + y])) : fmaxf(m4[y], v[x + y]);
         }
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+        const float mx = below_max<E, STEP>(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2);
         if (i == u.i0) {
           m = mx;
         } else {
-          const bool raise = mx > m + 8.f;
+          const bool raise = mx > m + STEP;
           if (__any_sync(0xFFFFFFFFu, raise)) {
             // the product of the tile before adds to the sum
             if (!warp_wait(o_done + NBUF * t + (tn - 1) % NBUF, (tn - 1) / NBUF)) {
