@@ -62,6 +62,10 @@ SSB_DEV Seq seq_of(const Args& a, int b) {
   return s;
 }
 
+// First token inside the window of a query at position p. Queries before the sequence's start have negative positions and
+// see nothing; taken as position 0, the difference stays inside 32 bits for any window.
+SSB_DEV int window_start(const Args& a, int p) { return max(max(p, 0) - a.window + 1, 0); }
+
 // The tiles of T tokens that rows at positions p_min .. p_max can see: the sinks' first, then the window's. A range
 // without a visible token has one (fully masked) tile, so that its rows are still written.
 struct Range {
@@ -70,7 +74,7 @@ struct Range {
 SSB_DEV Range range_of(const Args& a, int p_min, int p_max, int T) {
   Range r;
   const int end = p_max < 0 ? 0 : p_max / T + 1;
-  r.first = a.window ? max(p_min - a.window + 1, 0) / T : 0;
+  r.first = a.window ? window_start(a, p_min) / T : 0;
   r.first = min(r.first, end);
   r.sink_tiles = min((a.sinks + T - 1) / T, r.first);
   r.tiles = max(r.sink_tiles + end - r.first, 1);

@@ -350,7 +350,7 @@ SSB_DEV void tmem_ld_row(uint32_t taddr, float* v) {
 SSB_DEV uint32_t bits_below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
 SSB_DEV uint32_t seen_bits(const Args& a, int p, int t0) {
   uint32_t m = bits_below(p + 1 - t0);
-  if (a.window) m &= ~bits_below(p - a.window + 1 - t0) | bits_below(a.sinks - t0);
+  if (a.window) m &= ~bits_below(window_start(a, p) - t0) | bits_below(a.sinks - t0);
   return m;
 }
 SSB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
