@@ -437,8 +437,8 @@ int ssb_gemv_dense(const void* x, int32_t x_dtype, int64_t rows, const uint16_t*
  * s, or -1. refs[p] counts the table entries that hold page p; bit p % 32 of free_words[p / 32] is set exactly while
  * refs[p] is 0 (bits past `pages` are 0). lengths[s] = tokens of sequence s. All state is caller-owned device memory,
  * read and changed in stream order: no call waits for the host, so calls can be captured. err gets SSB_ERR_* bits.
- * scratch: int32 [ssb_kv_scratch_ints(pages, seqs)], set to zero once by the caller and left alone afterwards (it holds
- * which sequences wait for room); calls sharing a cache must not overlap. seqs <= 65536, pages <= 2^20, page_bytes a multiple of 16, pool 16-byte aligned. */
+ * scratch: int32 [ssb_kv_scratch_ints(pages, seqs)], set to zero once by the caller and left alone afterwards (it holds,
+ * among others, which sequences wait for room); calls sharing a cache must not overlap. seqs <= 65536, pages <= 2^20, page_bytes a multiple of 16, pool 16-byte aligned. */
 typedef struct ssb_kv_cache {
   void* pool;
   int64_t page_bytes;
@@ -478,7 +478,8 @@ int ssb_kv_write(const ssb_kv_cache* c, const ssb_kv_rows* r, void* stream);
 
 /* children[i] becomes a copy of parents[i] (i < n): full pages are shared (refs + 1), a partly filled last page is
  * copied to a fresh page (the lowest free ones, in the order of i), so that either can be extended. A child must be
- * empty (length 0, no pages) and named once; a parent may have many children. All or nothing, as ssb_kv_extend. */
+ * empty (length 0, no page in its first entry nor in any that it gets) and named once; a parent may have many children. All or
+ * nothing, as ssb_kv_extend. */
 int ssb_kv_fork(const ssb_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
 
 /* Gives pages back: a page whose last reference goes becomes free. first / last NULL: every page of ids[i], whose
