@@ -26,7 +26,9 @@ _ERRORS = {_lib.ERR_NO_PAGES: "not enough free pages, or a table row is full",
            _lib.ERR_SEQUENCE: "a sequence id out of range or repeated, a bad count, or a fork onto a held sequence",
            _lib.ERR_PAGE_RANGE: "a missing page or one outside the pool",
            _lib.ERR_SHARED_PAGE: "new tokens in a page that another sequence holds too",
-           _lib.ERR_NO_ROOM: "rows for a sequence whose last extend was refused, which were dropped"}
+           _lib.ERR_NO_ROOM: "rows for a sequence whose last extend was refused, which were dropped",
+           _lib.ERR_TIMEOUT: "a wait inside a prompt's attention gave up, and rows of its output were not written",
+           _lib.ERR_MISALIGNED: "the prompt attention kernel's shared memory was not aligned, and no output was written"}
 
 
 def state_ints(pages: int, seqs: int, max_pages: int) -> int:
@@ -162,5 +164,7 @@ class PagedKvCache:
         bits = int(self.err.item())
         if bits:
             self.err.zero_()
-            raise RuntimeError("kv cache: " + "; ".join(m for b, m in _ERRORS.items() if bits & b) +
-                               f" (error bits {bits})")
+            known = [m for b, m in _ERRORS.items() if bits & b]
+            if bits & ~sum(_ERRORS):
+                known.append("an unknown error")
+            raise RuntimeError("kv cache: " + "; ".join(known) + f" (error bits {bits})")
