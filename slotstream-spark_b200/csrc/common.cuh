@@ -58,9 +58,10 @@ SSB_DEV uint32_t lanemask_lt() {
 
 // ---------------------------------------------------------------- PDL (griddepcontrol, sm_90+)
 // pdl_wait: block until the grids this one depends on have completed and their writes are visible.
-// pdl_trigger: allow the next PDL-launched grid in the stream to start its prologue. Every kernel here calls
-// pdl_trigger only after pdl_wait, so a grid that starts early can rely on everything two launches back
-// being complete. Both are no-ops when the kernel was launched without the PDL attribute.
+// pdl_trigger: allow the next PDL-launched grid in the stream to start its prologue. A kernel that is launched with the
+// PDL attribute calls pdl_trigger only after pdl_wait (one launched without it starts when all before it has ended, and may
+// trigger at once), so a grid that starts early can rely on everything two launches back being complete. pdl_wait is a
+// no-op in a kernel launched without the attribute, pdl_trigger where the next grid is.
 SSB_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 SSB_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

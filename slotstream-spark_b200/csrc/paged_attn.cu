@@ -1,8 +1,9 @@
 // Attention over the paged key-value cache for few query rows per key head: decode steps and speculative verifies.
 //
 // Per item (sequence, key head, block of RB query rows): s = q k^T, online softmax (running maximum and sum, fp32,
-// log2 domain), o = p v. The rows of one key head -- query tokens x heads of its group -- share every key and value
-// read, so each cached byte is read once per key head: the kernel is bound by reading the cache. Tensor cores
+// log2 domain), o = p v. Up to 16 rows of one key head -- query tokens x heads of its group -- share every key and value
+// read, so up to there each cached byte is read once per key head: the kernel is bound by reading the cache. More rows (a
+// verify of four tokens of a group of eight, say) are several items, and each of them reads the cache again. Tensor cores
 // (mma.sync m16n8k16, fp32 accumulation) do both products, since RB x D x 2 multiply-adds per cached element pair
 // would otherwise take more issue slots than the loads leave; tcgen05's 128-row tiles would be mostly padding here. The
 // products are taken transposed -- S^T = K Q^T, O^T = V^T P^T -- so that the query rows are the instruction's 8 columns
@@ -564,7 +565,8 @@ Layout layout_of(int blocks, int rows, int dim) {
 // has at most DIRECT_GOOD tiles or the GPU is full; more than DIRECT_MOST tiles a block, or more than DIRECT_WAVES fillings
 // of the GPU, go the other way. Device time, whole items against split (16 heads, 2 key heads, head size 256): 16 sequences of
 // 1,000 tokens 12.8 against 13.9 us, 64 of 500 19.7 against 22.7, one of 2,000 12.5 against 11.2 (but one launch less, 4 us
-// of host time); 24 heads, 8 key heads, head size 64, 256 sequences of 500: 70 against 59.
+// of host time, which a captured call does not have: there the rule loses the 1.3 us); 24 heads, 8 key heads, head size 64,
+// 256 sequences of 500: 70 against 59.
 constexpr int DIRECT_GOOD = 4, DIRECT_MOST = 8, DIRECT_WAVES = 4;
 int tiles_at_most(const Args& a, int tile) {
   int64_t len = (int64_t)a.max_pages * a.page_size;

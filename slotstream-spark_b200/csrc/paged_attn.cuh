@@ -1,11 +1,16 @@
-// Shared pieces of the attention kernels over the paged key-value cache: arguments, visible-tile ranges, the split of
-// the work over blocks and the join of the pieces.
+// Shared pieces of the attention kernels over the paged key-value cache: arguments, sequences, visible-tile ranges, the
+// rounding of the weights.
 //
 // Work is a list of items -- (sequence, key head, block of query rows) -- each a run of tiles of the tokens it can
-// see. The total number of tiles is divided evenly over the blocks, whatever the lengths: block c takes tiles
-// [c * chunk, (c + 1) * chunk) of the concatenated items. An item inside one block is finished there; one that crosses
-// blocks leaves (max, sum, accumulator) pieces in the workspace, which k_attn_join sums in block order. The split
-// depends on the lengths alone, so results do not change from run to run.
+// see. How they are divided:
+// - few rows, long items (paged_attn.cu, k_attn_rows<DIRECT = false>): the total number of tiles evenly over the blocks,
+//   whatever the lengths: block c takes tiles [c * chunk, (c + 1) * chunk) of the concatenated items. An item inside one
+//   block is finished there; one that crosses blocks leaves (max, sum, accumulator) pieces in the workspace, which
+//   k_attn_join sums in block order.
+// - few rows, short items (DIRECT): a cluster of one to eight blocks an item, joined in rank order through shared memory.
+// - prompts (paged_prefill.cu): a planned list of whole items and pieces of items, taken by a counter; k_prefill_join sums
+//   the pieces of an item in their order.
+// In each case what is summed with what depends on the lengths alone, so results do not change from run to run.
 #pragma once
 #include <type_traits>
 
@@ -33,8 +38,8 @@ struct Args {
   int32_t* err;
   int4* desc;                         // items to join (see k_attn_join)
   int desc_by_item;
-  float2* ml;                         // [2 * blocks, RB] (max, sum) of the pieces, log2 domain
-  float* acc;                         // [2 * blocks, RB, D]
+  float2* ml;                         // (max, sum) of the pieces' rows, log2 domain: [2 * blocks, RB], or [slots, MB] for prompts
+  float* acc;                         // their accumulators, D floats a row
 };
 
 SSB_DEV int page_of(const Args& a, int t) { return (int)((__umulhi((uint32_t)t, a.page_mul) + (uint32_t)t) >> a.page_shift); }

@@ -24,15 +24,19 @@
 // Tiles of 64 tokens: two buffers of S for two row tiles of head size 128 fill TMEM. Instructions of 64 columns cost 48
 // cycles for 32 columns' worth of work (operands read from shared memory), so the products of a pair of tiles take 2570
 // cycles per 128 tokens instead of 2050; single-buffered tiles of 128, where each S waits for the product before it, took
-// 4600 (32K tokens, 32 heads, 8 key heads, window 4096: 2.16 ms against 1.91, 1.08 PFLOP/s). At size 256 two chunks of 2,048
-// tokens after 14K and 3K take 0.61 ms (1.05 PFLOP/s): each tile brings 64 KB of K and V for one row tile, 8 TB/s out of L2 through a
-// ring of only five slots, and shared memory moves 192 KB for it. Without the exponentials it takes as long, with half of
-// Q K^T left out 0.52 (10 TB/s); the scores of two tiles in one instruction of 128 columns hold two slots at once: 0.68.
+// 4600 (32K tokens, 32 heads, 8 key heads, window 4096: 2.16 ms against 1.91). At size 256 two chunks of 2,048 tokens after
+// 14K and 3K take 0.61 ms: each tile brings 64 KB of K and V for one row tile, 8 TB/s out of L2 through a ring of only five
+// slots, and shared memory moves 192 KB for it. Without the exponentials it takes as long, with half of Q K^T left out 0.52
+// (10 TB/s); the scores of two tiles in one instruction of 128 columns hold two slots at once: 0.68. These are single bursts at
+// full clocks (1.08 and 1.05 PFLOP/s); call after call, under the power cap, the two cases take 2.26 and 0.70 ms (0.92 and 0.90).
 //
 // Balance: k_prefill_plan lists the items, longest first within a sequence, cut into pieces that shrink with the work left
 // (an item of w tiles with R tiles left, itself included, and C blocks: pieces of about max(R / C, total / 16 C)); blocks
-// take units from the list by a counter. Only the items of the last wave or so are cut, and k_prefill_join sums their
-// pieces in order, so the outcome does not depend on who took which.
+// take units from the list by a counter; k_prefill_join sums an item's pieces in order, so the outcome does not depend on who
+// took which. Where there are many more items than blocks only those of the last wave or so are cut. With about 64 to 140 items
+// all of them are, and the pieces wanted can pass the 4 C slots that there are: then an item near the end of the list stays
+// whole, and one block works alone for longest (restated on the CPU: 1,024 tokens after 100,000, 32 heads, 8 key heads, size 128,
+// 128 items: 617 pieces wanted, 2,863 tiles in the longest block where an even split has 1,359).
 #include "paged_attn.cuh"
 
 #include "affine.cuh"
@@ -663,7 +667,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) k_prefill(const __grid_con
     while (ok && next_unit(u, WholeWarp())) {
       const Range rg = range_for(u);
       const int p = u.len - u.q, f0 = u.r0 + t * 128, last = u.r0 + u.rows - 1;
-      const int pos = p + min(f0 + row, last) / a.group;       // rows past the last: zero queries, never written
+      // rows past the last have zero queries or, where Q came in boxes, another sequence's; they are never written
+      const int pos = p + min(f0 + row, last) / a.group;
       const int t_lo = p + min(f0, last) / a.group, t_hi = p + min(f0 + 127, last) / a.group;
       float m = -INFINITY, l = 0.f;
       for (int i = u.i0; i < u.i1; ++i, ++tn) {

@@ -10,9 +10,9 @@ A query that sees nothing gives zeros and a log-sum-exp of -inf. ``ids`` (int32)
 
 Scores, softmax statistics and sums are fp32; the softmax weights are rounded to the inputs' type for the tensor cores.
 ``lse`` (fp32, optional output) is the natural log-sum-exp of the scaled scores, for joining with other parts. ``err``
-(int32 [1], e.g. ``PagedKvCache.err``) gets error bits; without it nothing tells of a missing page, a bad id or a prompt whose
-kernel gave up waiting (rows of ``out`` are then left unwritten), so a program passes it; ``ws`` (uint8, ``workspace_bytes``) avoids the allocation of a
-workspace, which capture in a CUDA graph with caller-owned memory wants."""
+(int32 [1], e.g. ``PagedKvCache.err``) gets error bits; without it nothing tells of a missing page, a bad id or a prompt
+whose kernel gave up waiting (rows of ``out`` are then left unwritten), so a program passes it; ``ws`` (uint8,
+``workspace_bytes``) avoids the allocation of a workspace, which capture in a CUDA graph with caller-owned memory wants."""
 import ctypes
 import math
 

@@ -8,9 +8,11 @@ contiguous run of bytes to copy, and ``k(layer)`` / ``v(layer)`` are strided vie
 
 All state is device memory and every call only launches on the current stream: nothing waits for the host, and the calls
 can be captured in a CUDA graph. What the device finds wrong -- no free pages, a bad or repeated sequence, a shared page
-about to be written -- leaves the state as it was and sets a bit in ``err``; ``check()`` reads it (and waits for it). After
-an ``extend`` that was refused, ``write`` drops the rows of the sequences that it named until an ``extend`` has made room for
-them, so that a step need not look in between; the attention of that step then sees the tokens of before.
+about to be written -- sets a bit in ``err``; ``check()`` reads it (and waits for it). ``extend`` and ``fork`` then leave the
+state as it was; ``free`` and ``release`` pass over bad ids, and ``write`` drops the rows that have no place. After an
+``extend`` that was refused, ``write`` drops the rows of the sequences that it was to give room, until an ``extend`` has made
+it, so that a step need not look in between; the attention of that step sees the tokens of before. Which sequences wait for
+room is kept in ``scratch``, so calls that belong together go through one ``PagedKvCache``.
 
 A decode step: ``extend(ids, counts)`` once (lengths grow, pages are allocated), then per layer ``write(layer, k, v,
 starts, ids)``, ``attn_decode(q, cache.k(layer), cache.v(layer), cache.table, cache.lengths, ids=ids)`` and the MoE layer.
